@@ -19,9 +19,11 @@ LIB = PACKAGE_DIR / "lib" / "libodf_sm100.so"
 # The same sources with the in-kernel invariant checks compiled in (-DODF_CHECKED): test
 # infrastructure (tests/test_checked_build_gpu.py), never loaded by the package itself.
 CHECKED_LIB = PACKAGE_DIR / "lib" / "libodf_sm100_checked.so"
-SOURCES = [CSRC / "flash_fwd_sm100.cu", CSRC / "odf_capi.cu"]
+SOURCES = [CSRC / "flash_fwd_sm100.cu", CSRC / "odf_capi.cu", CSRC / "paged_sm100.cu", CSRC / "paged_capi.cpp",
+           CSRC / "page_pool.cpp"]
 CXX_API_SOURCES = [CSRC / "onednn_flash_api.cpp", CSRC / "planner.cpp"]
-DEPS = SOURCES + CXX_API_SOURCES + [CSRC / "sm100_ptx.cuh", CSRC / "softmax_math.cuh", CSRC / "odf_internal.h"] + sorted(
+DEPS = SOURCES + CXX_API_SOURCES + [CSRC / "sm100_ptx.cuh", CSRC / "softmax_math.cuh", CSRC / "odf_internal.h",
+                                   CSRC / "paged_internal.h"] + sorted(
     (ROOT / "include").rglob("*.h*"))
 # Test-only device wrappers of the softmax arithmetic helpers (error-bound tests).
 MATH_CHECK_SRC = ROOT / "tests" / "cuda" / "math_check.cu"

@@ -143,9 +143,7 @@ size_t workspace_with_far_bound(const odf_fwd_params* p, int64_t batch, int64_t 
     return bytes;
 }
 
-float generated_slope(int64_t h, int64_t heads) {
-    return std::exp2(-8.0f * static_cast<float>(h + 1) / static_cast<float>(heads));
-}
+float generated_slope(int64_t h, int64_t heads) { return odf::generated_alibi_slope(h, heads); }
 
 odf::FwdLaunch make_launch(const odf_fwd_params* p, const Resolved& r) {
     odf::FwdLaunch L;
@@ -314,6 +312,22 @@ struct HostPool {
 thread_local HostPool t_pool;
 
 }  // namespace
+
+namespace odf {
+
+int set_error(int code, const char* msg) noexcept {
+    try {
+        t_last_error = msg;
+    } catch (...) {  // out of memory: the status code stands alone
+    }
+    return code;
+}
+
+float generated_alibi_slope(int64_t h, int64_t heads) {
+    return std::exp2(-8.0f * static_cast<float>(h + 1) / static_cast<float>(heads));
+}
+
+}  // namespace odf
 
 extern "C" {
 

@@ -187,4 +187,10 @@ size_t kv_split_bytes(int64_t batch, int64_t heads_q, int64_t seqlen_q, int64_t 
 // uses for its far-tile bound (tile norms and the per-pair first visited KV tile).
 size_t far_bound_bytes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t seqlen_q, int64_t seqlen_k);
 
+// Keeps `msg` for odf_last_error on this thread and returns `code` (never throws).
+int set_error(int code, const char* msg) noexcept;
+
+// Generated ALiBi slope of head h of `heads` (the value every entry uses up to 256 heads).
+float generated_alibi_slope(int64_t h, int64_t heads);
+
 }  // namespace odf

@@ -25,8 +25,11 @@ ODF_ERR_UNSUPPORTED = 2
 ODF_ERR_CUDA = 3
 ODF_ERR_DEVICE_TIMEOUT = 4
 ODF_ERR_NO_DEVICE = 5
+ODF_ERR_BAD_PAGE = 7
+ODF_ERR_NO_PAGES = 8
 ODF_DTYPE_F32 = 0
 ODF_DTYPE_BF16 = 1
+ODF_DTYPE_E4M3 = 16
 ODF_BIAS_NONE = 0
 ODF_BIAS_SAME_SHAPE = 1
 ODF_BIAS_ALIBI = 4
@@ -49,6 +52,41 @@ class FwdParams(C.Structure):
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
         ("tile_visits", C.c_void_p),
         ("bias", C.c_void_p), ("bias_strides", C.c_int64 * 4),
+    ]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("kv_dtype", C.c_int32),
+        ("num_pages", C.c_int64), ("heads_kv", C.c_int64), ("page_size", C.c_int64), ("head_dim", C.c_int64),
+        ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("max_pages", C.c_int64),
+    ]
+
+
+class DecodeParams(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p), ("o_dtype", C.c_int32),
+        ("batch", C.c_int64), ("heads_q", C.c_int64), ("q_strides", C.c_int64 * 2), ("o_strides", C.c_int64 * 2),
+        ("lens", C.c_void_p), ("cache", PagedCache), ("scale", C.c_float), ("window", C.c_int64),
+        ("sinks", C.c_int64), ("bias_kind", C.c_int32), ("alibi_slopes", C.c_void_p), ("softcap", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class AppendParams(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("batch", C.c_int64), ("tokens", C.c_int64),
+        ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3),
+        ("starts", C.c_void_p), ("counts", C.c_void_p), ("cache", PagedCache),
+    ]
+
+
+class PageCopyParams(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("layers", C.c_int64), ("k_layer_stride", C.c_int64), ("v_layer_stride", C.c_int64),
+        ("pairs", C.c_void_p), ("n_pairs", C.c_int64),
     ]
 
 
@@ -77,6 +115,25 @@ def load_library():
                                        C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]
     lib.odf_convert_f32_to_bf16.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
     lib.odf_device_status.argtypes = [C.POINTER(C.c_int32), C.c_int32]
+    lib.odf_paged_decode_sm100.argtypes = [C.POINTER(DecodeParams), C.c_void_p]
+    lib.odf_paged_decode_workspace_size.argtypes = [C.POINTER(DecodeParams)]
+    lib.odf_paged_decode_workspace_size.restype = C.c_size_t
+    lib.odf_paged_append_sm100.argtypes = [C.POINTER(AppendParams), C.c_void_p]
+    lib.odf_page_copy_sm100.argtypes = [C.POINTER(PageCopyParams), C.c_void_p]
+    i64, p64, p32 = C.c_int64, C.POINTER(C.c_int64), C.c_void_p
+    lib.odf_page_pool_create.argtypes = [i64, i64, C.POINTER(C.c_void_p)]
+    lib.odf_page_pool_destroy.argtypes = [C.c_void_p]
+    lib.odf_page_pool_destroy.restype = None
+    lib.odf_page_pool_add.argtypes = [C.c_void_p, p64]
+    lib.odf_page_pool_fork.argtypes = [C.c_void_p, i64, p64]
+    lib.odf_page_pool_extend.argtypes = [C.c_void_p, i64, i64, p32, p64]
+    lib.odf_page_pool_truncate.argtypes = [C.c_void_p, i64, i64]
+    lib.odf_page_pool_free.argtypes = [C.c_void_p, i64]
+    lib.odf_page_pool_compact.argtypes = [C.c_void_p, p32, i64, p64]
+    lib.odf_page_pool_length.argtypes = [C.c_void_p, i64, p64, p64]
+    lib.odf_page_pool_table.argtypes = [C.c_void_p, i64, p32, i64]
+    lib.odf_page_pool_free_pages.argtypes = [C.c_void_p]
+    lib.odf_page_pool_free_pages.restype = i64
     lib.odf_last_error.restype = C.c_char_p
     lib.odf_version.restype = C.c_char_p
     _lib = lib
@@ -291,6 +348,323 @@ def tile_map(seqlen_q, seqlen_k, causal, block_mask=None, mask_block=(128, 128),
     _check(rc)
     torch.cuda.synchronize()
     return out
+
+
+# ------------------------------------------------------------------ paged key-value cache
+def _on(tensor, name, device):
+    if tensor is not None and tensor.device != device:
+        raise ValueError(f"{name} is on {tensor.device}, the call runs on {device}")
+
+
+def _int32_on(tensor, name, device, shape):
+    """A contiguous int32 device tensor of the given shape (None where a size is free)."""
+    import torch
+
+    _on(tensor, name, device)
+    if tensor.dtype != torch.int32 or tensor.dim() != len(shape) or any(
+            n is not None and n != m for n, m in zip(shape, tensor.shape)):
+        raise ValueError(f"{name} must be int32 of shape {list(shape)}, got {tensor.dtype} {list(tensor.shape)}")
+    if tensor.stride(-1) != 1 and tensor.shape[-1] > 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    return tensor.data_ptr()
+
+
+def _dense_strides(t, name):
+    """Strides of all dimensions but the last, which must be contiguous.  A dimension of size 1 has
+    no stride of its own; it gets the one a contiguous tensor would have."""
+    if t.stride(-1) != 1:
+        raise ValueError(f"the innermost (feature) dimension of {name} must be contiguous")
+    out, dense = [], 1
+    for n, s in zip(reversed(t.shape), reversed(t.stride())):
+        out.append(dense if n == 1 else s)
+        dense *= n
+    return list(reversed(out))[:-1]
+
+
+def _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, batch):
+    import torch
+
+    if k_pages.dim() != 4 or v_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must be rank 4 [pages, heads_kv, page_size, head_dim] of one shape")
+    if k_pages.dtype != v_pages.dtype:
+        raise ValueError("k_pages and v_pages must have one dtype")
+    c = PagedCache()
+    c.k_pages, c.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
+    if k_pages.dtype == torch.bfloat16:
+        c.kv_dtype = ODF_DTYPE_BF16
+    elif k_pages.dtype == torch.float8_e4m3fn:
+        c.kv_dtype = ODF_DTYPE_E4M3
+    else:
+        raise ValueError(f"a cache holds bfloat16 or float8_e4m3fn, not {k_pages.dtype}")
+    dev = k_pages.device
+    _on(v_pages, "v_pages", dev)
+    c.num_pages, c.heads_kv, c.page_size, c.head_dim = k_pages.shape
+    for field, t, name in ((c.k_strides, k_pages, "k_pages"), (c.v_strides, v_pages, "v_pages")):
+        for i, s in enumerate(_dense_strides(t, name)):
+            field[i] = s
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t is not None:
+            _on(t, name, dev)
+            if t.dtype != torch.float32 or t.shape != (c.heads_kv,) or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous float32 tensor [heads_kv]")
+            setattr(c, name, t.data_ptr())
+    if page_table is not None:
+        c.page_table = _int32_on(page_table, "page_table", dev, (batch, None))
+        c.max_pages = page_table.shape[1]
+        c.table_stride = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
+    return c
+
+
+class _launch_on:
+    """Makes `device` current and yields the stream handle to launch on; temporaries and outputs
+    allocated inside belong to that stream."""
+
+    def __init__(self, device, stream):
+        import torch
+
+        self.device = torch.cuda.device(device)
+        current = torch.cuda.current_stream(device)
+        self.handle = current.cuda_stream if stream is None else getattr(stream, "cuda_stream", stream)
+        self.stream = None
+        if self.handle != current.cuda_stream:
+            self.stream = torch.cuda.stream(torch.cuda.ExternalStream(self.handle, device=device) if self.handle
+                                            else torch.cuda.default_stream(device))
+
+    def __enter__(self):
+        self.device.__enter__()
+        if self.stream is not None:
+            self.stream.__enter__()
+        return C.c_void_p(self.handle)
+
+    def __exit__(self, *exc):
+        if self.stream is not None:
+            self.stream.__exit__(*exc)
+        return self.device.__exit__(*exc)
+
+
+def _require_cuda(device):
+    if device.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, not {device}")
+
+
+def paged_decode_workspace(batch, heads_q, heads_kv, head_dim, device="cuda"):
+    """Scratch for ``paged_decode``, zeroed: a serving loop keeps one per stream for all of its calls."""
+    import torch
+
+    p = DecodeParams()
+    p.batch, p.heads_q, p.cache.heads_kv, p.cache.head_dim = batch, heads_q, heads_kv, head_dim
+    return torch.zeros(load_library().odf_paged_decode_workspace_size(C.byref(p)), dtype=torch.uint8, device=device)
+
+
+def paged_decode(q, k_pages, v_pages, page_table, lens, *, scale=None, window=0, sinks=0, alibi=False,
+                 alibi_slopes=None, softcap=0.0, k_scale=None, v_scale=None, out_dtype=None, want_lse=True, out=None,
+                 lse_out=None, workspace=None, stream=None):
+    """Attention of one new token per sequence over a paged cache (odf_paged_decode_sm100).
+
+    q [B,Hq,D] bf16; k_pages, v_pages [pages,Hkv,page_size,D] bf16 or float8_e4m3fn (any strides that are
+    multiples of 16 bytes, so a [pages,page_size,Hkv,D] cache goes in as a ``transpose(1, 2)`` view);
+    page_table int32 [B,max_pages]; lens int32 [B], keys per sequence with the new token's own (append
+    first).  ``window`` > 0 keeps the last ``window`` keys and the first ``sinks``.  ``workspace``:
+    ``paged_decode_workspace(...)``, kept between calls on one stream; without one, each call makes its own.
+
+    Returns (o [B,Hq,D], lse [B,Hq] fp32 natural log, or None), asynchronous on ``stream``
+    (default: torch's current stream).
+    """
+    import torch
+
+    lib = load_library()
+    if q.dim() != 3 or q.dtype != torch.bfloat16:
+        raise ValueError("q must be bfloat16 of rank 3 [B, Hq, D]")
+    B, Hq, D = q.shape
+    dev = q.device
+    _require_cuda(dev)
+    _on(k_pages, "k_pages", dev)
+    if k_pages.dim() == 4 and k_pages.shape[3] != D:
+        raise ValueError("q and the cache must have one head_dim")
+    p = DecodeParams()
+    p.cache = _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, B)
+    p.q, p.lens = q.data_ptr(), _int32_on(lens, "lens", dev, (B,))
+    p.batch, p.heads_q = B, Hq
+    p.scale = 1.0 / math.sqrt(D) if scale is None else scale
+    p.window, p.sinks, p.softcap = window, sinks, softcap
+    keep = None
+    if alibi:
+        p.bias_kind = ODF_BIAS_ALIBI
+        if alibi_slopes is not None:
+            if len(alibi_slopes) != Hq:
+                raise ValueError("alibi_slopes needs one slope per query head")
+            keep = (C.c_float * Hq)(*[float(x) for x in alibi_slopes])
+            p.alibi_slopes = C.cast(keep, C.c_void_p)
+    with _launch_on(dev, stream) as handle:
+        if out is None:
+            out = torch.empty((B, Hq, D), dtype=out_dtype or torch.float32, device=dev)
+        lse = lse_out
+        if want_lse and lse is None:
+            lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
+        _on(out, "out", dev)
+        _on(lse, "lse_out", dev)
+        if out.shape != q.shape or out.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("out must be float32 or bfloat16 of q's shape")
+        if lse is not None and (lse.shape != (B, Hq) or lse.dtype != torch.float32 or not lse.is_contiguous()):
+            raise ValueError("lse_out must be contiguous float32 [B, Hq]")
+        p.o, p.o_dtype = out.data_ptr(), ODF_DTYPE_BF16 if out.dtype == torch.bfloat16 else ODF_DTYPE_F32
+        p.lse = lse.data_ptr() if lse is not None else None
+        for field, t, name in ((p.q_strides, q, "q"), (p.o_strides, out, "out")):
+            for i, s in enumerate(_dense_strides(t, name)):
+                field[i] = s
+        if workspace is None:
+            workspace = paged_decode_workspace(B, Hq, p.cache.heads_kv, D, device=dev)
+        _on(workspace, "workspace", dev)
+        p.workspace, p.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        _check(lib.odf_paged_decode_sm100(C.byref(p), handle))
+    del keep
+    return out, (lse if want_lse else None)
+
+
+def paged_append(k, v, k_pages, v_pages, page_table, starts, *, counts=None, k_scale=None, v_scale=None, stream=None):
+    """Writes k, v [B,Hkv,T,D] (bf16) into the cache at positions starts[b] .. (odf_paged_append_sm100).
+
+    Token t of sequence b is written when t < counts[b] (always without ``counts``, int32 [B]).  A
+    float8_e4m3fn cache gets x / scale, rounded to nearest and saturated.  Asynchronous on ``stream``.
+    """
+    import torch
+
+    lib = load_library()
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise ValueError("k and v must be bfloat16 of one rank 4 shape [B, Hkv, T, D]")
+    B, Hkv, T, D = k.shape
+    dev = k.device
+    _require_cuda(dev)
+    _on(v, "v", dev)
+    _on(k_pages, "k_pages", dev)
+    if k_pages.dim() == 4 and (k_pages.shape[1] != Hkv or k_pages.shape[3] != D):
+        raise ValueError("k and the cache must have the same kv-heads and head_dim")
+    p = AppendParams()
+    p.cache = _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, B)
+    p.k, p.v, p.batch, p.tokens = k.data_ptr(), v.data_ptr(), B, T
+    for field, t, name in ((p.k_strides, k, "k"), (p.v_strides, v, "v")):
+        for i, s in enumerate(_dense_strides(t, name)):
+            field[i] = s
+    p.starts = _int32_on(starts, "starts", dev, (B,))
+    p.counts = _int32_on(counts, "counts", dev, (B,)) if counts is not None else None
+    with _launch_on(dev, stream) as handle:
+        _check(lib.odf_paged_append_sm100(C.byref(p), handle))
+
+
+def page_copy(k_pages, v_pages, pairs, *, stream=None):
+    """Copies pages pairs[i] = (source, destination) of K and V (odf_page_copy_sm100).
+
+    k_pages, v_pages: one layer [pages,Hkv,page_size,D], or every layer [layers,pages,Hkv,page_size,D] in one
+    launch.  ``pairs``: a sequence of pairs, a numpy array or a CPU tensor [n,2], such as
+    ``PagePool`` gives out.  Asynchronous on ``stream``.
+    """
+    import numpy as np
+
+    lib = load_library()
+    if k_pages.dim() not in (4, 5) or k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must be [pages, Hkv, page_size, D] or [layers, pages, ...] of one shape")
+    dev = k_pages.device
+    _require_cuda(dev)
+    ids = np.asarray(pairs)
+    if ids.size == 0:
+        ids = np.zeros((0, 2), dtype=np.int32)
+    if ids.ndim != 2 or ids.shape[1] != 2 or not np.issubdtype(ids.dtype, np.integer):
+        raise ValueError("pairs must be integers of shape [n, 2]")
+    if ids.size and (ids.min() < 0 or ids.max() >= k_pages.shape[-4]):
+        raise ValueError("a page id is outside the cache")
+    ids = np.ascontiguousarray(ids, dtype=np.int32)
+    p = PageCopyParams()
+    layered = k_pages.dim() == 5
+    if layered and k_pages.shape[0] == 0:
+        raise ValueError("the cache has no layers")
+    p.cache = _cache_params(k_pages[0] if layered else k_pages, v_pages[0] if layered else v_pages, None, None, None, 0)
+    p.layers = k_pages.shape[0] if layered else 1
+    if layered:
+        p.k_layer_stride, p.v_layer_stride = k_pages.stride(0), v_pages.stride(0)
+    p.pairs, p.n_pairs = ids.ctypes.data, len(ids)
+    with _launch_on(dev, stream) as handle:
+        _check(lib.odf_page_copy_sm100(C.byref(p), handle))
+
+
+class PagePool:
+    """Which pages of a cache are free, and every sequence's table (odf_page_pool_*; host only).
+
+    ``extend`` and ``compact`` return (source, destination) pairs for ``page_copy``, to be run before the
+    cache is written or the pool changed again.  Not thread-safe.
+    """
+
+    def __init__(self, num_pages: int, page_size: int):
+        self._lib = load_library()
+        self._pool = C.c_void_p()
+        _check(self._lib.odf_page_pool_create(num_pages, page_size, C.byref(self._pool)))
+        self.num_pages, self.page_size = num_pages, page_size
+
+    def __del__(self):
+        if getattr(self, "_pool", None):
+            self._lib.odf_page_pool_destroy(self._pool)
+            self._pool = None
+
+    def add(self) -> int:
+        """A new, empty sequence."""
+        seq = C.c_int64()
+        _check(self._lib.odf_page_pool_add(self._pool, C.byref(seq)))
+        return seq.value
+
+    def fork(self, seq: int) -> int:
+        """A new sequence with the same tokens; every page is shared until one of the two writes it."""
+        child = C.c_int64()
+        _check(self._lib.odf_page_pool_fork(self._pool, seq, C.byref(child)))
+        return child.value
+
+    def extend(self, seq: int, tokens: int) -> list[tuple[int, int]]:
+        """Room for ``tokens`` more tokens; raises OdfError(ODF_ERR_NO_PAGES), changing nothing, without it."""
+        pair, n = (C.c_int32 * 2)(), C.c_int64()
+        _check(self._lib.odf_page_pool_extend(self._pool, seq, tokens, pair, C.byref(n)))
+        return [(pair[0], pair[1])] if n.value else []
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Drops the tokens past ``length``."""
+        _check(self._lib.odf_page_pool_truncate(self._pool, seq, length))
+
+    def free(self, seq: int) -> None:
+        """Ends a sequence."""
+        _check(self._lib.odf_page_pool_free(self._pool, seq))
+
+    def compact(self) -> list[tuple[int, int]]:
+        """Moves pages so that the used ones are the first ones."""
+        room = self.num_pages // 2
+        pairs, n = (C.c_int32 * (2 * max(room, 1)))(), C.c_int64()
+        _check(self._lib.odf_page_pool_compact(self._pool, pairs, room, C.byref(n)))
+        return [(pairs[2 * i], pairs[2 * i + 1]) for i in range(n.value)]
+
+    def length(self, seq: int) -> int:
+        tokens, pages = C.c_int64(), C.c_int64()
+        _check(self._lib.odf_page_pool_length(self._pool, seq, C.byref(tokens), C.byref(pages)))
+        return tokens.value
+
+    def pages(self, seq: int) -> list[int]:
+        tokens, pages = C.c_int64(), C.c_int64()
+        _check(self._lib.odf_page_pool_length(self._pool, seq, C.byref(tokens), C.byref(pages)))
+        ids = (C.c_int32 * max(pages.value, 1))()
+        _check(self._lib.odf_page_pool_table(self._pool, seq, ids, pages.value))
+        return list(ids[:pages.value])
+
+    def table(self, seqs, max_pages: int | None = None):
+        """The page table of a batch: int32 CPU tensor [len(seqs), max_pages], -1 past each sequence's pages."""
+        import torch
+
+        rows = [self.pages(s) for s in seqs]
+        width = max([1] + [len(r) for r in rows]) if max_pages is None else max_pages
+        out = torch.full((len(rows), width), -1, dtype=torch.int32)
+        for i, r in enumerate(rows):
+            if len(r) > width:
+                raise ValueError("a sequence has more pages than the table has entries")
+            out[i, :len(r)] = torch.tensor(r, dtype=torch.int32)
+        return out
+
+    @property
+    def free_pages(self) -> int:
+        return self._lib.odf_page_pool_free_pages(self._pool)
 
 
 def device_status(clear=True) -> int:
