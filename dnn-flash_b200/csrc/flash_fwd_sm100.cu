@@ -47,6 +47,7 @@
 #include <cudaTypedefs.h>
 
 #include <math.h>
+#include <algorithm>
 #include <mutex>
 
 #include "odf_internal.h"
@@ -120,8 +121,19 @@ __device__ __noinline__ void check_failed(int bit, int* status) {
 
 // Score-mod variants: ALiBi and the same-shape bias are exclusive (one BiasKind per call).
 // kModSkipMax marks the plain-score variant for long KV ranges whose unmasked tiles skip the
-// row-max pass (the low three bits select the score mods).
-enum ModFlags { kModAlibi = 1, kModSoftcap = 2, kModBias = 4, kModSkipMax = 8 };
+// row-max pass (the low three bits select the score mods).  kModWindow marks the sliding-window
+// variants (with any of the other flags but the bias).
+enum ModFlags { kModAlibi = 1, kModSoftcap = 2, kModBias = 4, kModSkipMax = 8, kModWindow = 16 };
+
+// Sliding-window variants: K and V maps that end at the last sink, so the sink tile of an item
+// whose window starts further on reads zeros past it (what lies between sinks and window may
+// have been evicted and hold anything).
+template <bool kWin>
+struct SinkMaps {};
+template <>
+struct SinkMaps<true> {
+    CUtensorMap k, v;
+};
 
 template <int D>
 struct Config {
@@ -204,13 +216,48 @@ struct Item {
     int n_entries;     // KV tiles visited by the pair (entries 0 .. n_entries - 1 of kv_entry)
     bool valid1;       // Q1 has rows
     int split, kv0;    // KV split of the item and its first KV tile (0, 0 without splits)
+    int win_lo, n_sink;  // sliding window: first key of its tiles, and the sink tiles before them
 };
+
+// Sliding window.  Row qi sits at position p = q_offset + qi and sees the keys j <= p with
+// p - j < window or j < sinks.  A pair of query tiles visits n_sink tiles over the sinks, if its
+// window starts past them, then tiles of 128 keys from win_lo, the first key that its first row
+// sees: tiles start where the window does, not at multiples of 128, so a window of W keys costs
+// ceil((W + 255) / 128) tiles and no key that every row has behind it is read.
+struct WindowSpan {
+    int lo, n_sink, n_win;
+};
+
+__device__ __forceinline__ WindowSpan window_span(const FwdArgs& a, int q00, int qend) {
+    WindowSpan w;
+    const int hi = min(a.n, a.q_offset + qend);
+    w.lo = max(0, a.q_offset + q00 - a.window + 1);
+    const int s_end = min(a.sinks, hi);
+    w.n_sink = 0;
+    if (s_end > 0) {
+        if (w.lo > s_end)
+            w.n_sink = (s_end + kTileK - 1) / kTileK;
+        else
+            w.lo = 0;  // the window touches the sinks: one run of tiles from key 0
+    }
+    w.n_win = hi > w.lo ? (hi - w.lo + kTileK - 1) / kTileK : 0;
+    return w;
+}
+
+// First key of the pair's tile t, and whether a query tile with rows at positions [p0, pe) needs it.
+__device__ __forceinline__ int window_tile_start(int t, int lo, int n_sink) {
+    return t < n_sink ? t * kTileK : lo + (t - n_sink) * kTileK;
+}
+__device__ __forceinline__ bool window_tile_needed(const FwdArgs& a, int start, bool sink, int p0, int pe) {
+    return start < pe && (sink || start + kTileK > p0 - a.window + 1 || start < a.sinks);
+}
 
 // Items come in blocks of units_per_block (batch, kv-head) units: inside a block, item i is
 // query-tile pair n_pairs-1-i/(U G) (longest causal rows first) of q-head i mod (U G) of the
 // block (G = q-heads per kv-head).  A block's K/V fits in L2 while its CTAs stream through it.
 // With one block holding every unit this is plain pair-major order over all heads.  With KV
 // splits, the n_splits splits of a pair's key range are consecutive items.
+template <bool kWin>
 __device__ __forceinline__ Item decode_item(const FwdArgs& a, int64_t k) {
     Item I;
     I.split = 0;
@@ -281,7 +328,12 @@ __device__ __forceinline__ Item decode_item(const FwdArgs& a, int64_t k) {
     I.valid1 = I.q01 < a.m;
     I.qend0 = min(a.m, I.q00 + kTileQ);
     I.qend1 = I.valid1 ? min(a.m, I.q01 + kTileQ) : I.qend0;
-    if (a.mode == kModeList) {
+    if constexpr (kWin) {
+        const WindowSpan w = window_span(a, I.q00, I.qend1);
+        I.win_lo = w.lo;
+        I.n_sink = w.n_sink;
+        I.n_entries = w.n_sink + w.n_win;
+    } else if (a.mode == kModeList) {
         I.n_entries = a.tile_count[I.pair];
     } else if (a.mode == kModeCausal) {
         I.n_entries = min(a.n_kt, (I.qend1 + kTileK - 1) / kTileK);
@@ -294,7 +346,17 @@ __device__ __forceinline__ Item decode_item(const FwdArgs& a, int64_t k) {
     return I;
 }
 
+template <bool kWin>
 __device__ __forceinline__ uint32_t kv_entry(const FwdArgs& a, const Item& I, int j) {
+    if constexpr (kWin) {
+        const int t = I.kv0 + j;
+        const int start = window_tile_start(t, I.win_lo, I.n_sink);
+        const bool sink = t < I.n_sink;
+        uint32_t e = static_cast<uint32_t>(t);
+        if (window_tile_needed(a, start, sink, a.q_offset + I.q00, a.q_offset + I.qend0)) e |= kNeed0;
+        if (I.valid1 && window_tile_needed(a, start, sink, a.q_offset + I.q01, a.q_offset + I.qend1)) e |= kNeed1;
+        return e;
+    }
     return kv_entry(a, I.pair, j, I.valid1, I.qend0, I.qend1, I.kv0);
 }
 
@@ -317,6 +379,11 @@ __device__ __forceinline__ void store_zero_p(uint32_t p_addr) {
     ptx::tmem_st64_zero_nowait(p_addr);
     ptx::tmem_st_wait();
     ptx::tc_fence_before();
+}
+
+// The lowest n of 32 bits (n clamped to [0, 32]).
+__device__ __forceinline__ uint32_t bits_below(int n) {
+    return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
 }
 
 // Bits of the 128 columns [k0, k0+128) that the BlockMask allows for query row qi
@@ -358,16 +425,20 @@ __device__ __forceinline__ uint4 row_allow_bits(const FwdArgs& a, int qi, int k0
 #ifndef ODF_POLY_MASK_SOFTCAP
 #define ODF_POLY_MASK_SOFTCAP 0x80  // one pair in eight: best of 0, 1/8, 1/4, 3/8, 1/2 on c3 and soft-cap-only 8K
 #endif
+// Not in the sliding-window variants: a row with few keys has no others to average the
+// polynomial's 1e-4 out.
 template <int D, int MOD>
 __host__ __device__ constexpr uint32_t poly_exp2_mask() {
-    return D == 64 ? ODF_POLY_MASK_D64 : ((MOD & kModSoftcap) ? ODF_POLY_MASK_SOFTCAP : 0u);
+    return (MOD & kModWindow) ? 0u : D == 64 ? ODF_POLY_MASK_D64 : ((MOD & kModSoftcap) ? ODF_POLY_MASK_SOFTCAP : 0u);
 }
 
 template <int D, int MOD>
 __global__ void __launch_bounds__(kThreads, 1)
     flash_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ FwdArgs args) {
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ FwdArgs args,
+                     const __grid_constant__ SinkMaps<(MOD & kModWindow) != 0> sink_maps) {
     using Cfg = Config<D>;
+    constexpr bool kWin = (MOD & kModWindow) != 0;
     constexpr int kSlots = Cfg::kSlots;
 
     extern __shared__ uint8_t smem_raw[];
@@ -402,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Greedy item assignment is compiled into the plain d = 128 kernel (the shapes whose K/V
     // outgrows L2 and whose speed depends on it) and the ALiBi d = 128 kernels (whose items'
     // lengths vary by head once far tiles are left out); the other variants keep the fixed order.
-    constexpr bool kDyn = D == 128 && ((MOD & 7) == 0 || (MOD & (kModAlibi | kModBias)) == kModAlibi);
+    constexpr bool kDyn = D == 128 && !kWin && ((MOD & 7) == 0 || (MOD & (kModAlibi | kModBias)) == kModAlibi);
     volatile int64_t* item_q = reinterpret_cast<volatile int64_t*>(smem + Cfg::kOffQueue);
 
     if (threadIdx.x == 0) {
@@ -473,10 +544,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         k = static_item(n_items, it);  // every role computes the same sequence
                     }
                     if (k < 0) break;
-                    const Item I = decode_item(args, k);
+                    const Item I = decode_item<kWin>(args, k);
                     ODF_CHECK(I.pair >= 0 && I.pair < args.n_pairs && I.bh >= 0 &&
                                   I.bh < args.batch * args.heads_q && I.hk >= 0 && I.hk < args.heads_kv &&
-                                  I.n_entries >= 0 && I.n_entries <= args.n_kt,
+                                  I.n_entries >= 0 && I.n_entries <= args.n_kt + (kWin ? 1 : 0),
                               0);
                     ODF_CHECK(args.kv_lo == nullptr || I.n_entries >= 1, 5);
                     if (I.n_entries == 0) continue;
@@ -496,12 +567,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     ++q_loads;
                     for (int j = 0; ok && j < I.n_entries; ++j) {
-                        const int kt = static_cast<int>(kv_entry(args, I, j) & 0xFFFFu);
+                        const int kt = static_cast<int>(kv_entry<kWin>(args, I, j) & 0xFFFFu);
+                        int row0 = kt * kTileK;  // first key of the tile
+                        if constexpr (kWin) row0 = window_tile_start(kt, I.win_lo, I.n_sink);
 #ifdef ODF_CHECKED
                         {
-                            const uint32_t e_chk = kv_entry(args, I, j);
-                            ODF_CHECK(kt < args.n_kt && kt * kTileK < args.n && (e_chk & (kNeed0 | kNeed1)) != 0 &&
-                                          (I.valid1 || !(e_chk & kNeed1)),
+                            const uint32_t e_chk = kv_entry<kWin>(args, I, j);
+                            ODF_CHECK((kWin || kt < args.n_kt) && row0 >= 0 && row0 < args.n &&
+                                          (e_chk & (kNeed0 | kNeed1)) != 0 && (I.valid1 || !(e_chk & kNeed1)),
                                       1);
                         }
 #endif
@@ -517,9 +590,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 ptx::mbar_arrive_expect_tx(&bars.slot_full[s], Cfg::kTileBytes);
                                 const void* map =
                                     half == 0 ? static_cast<const void*>(&tmK) : static_cast<const void*>(&tmV);
+                                if constexpr (kWin) {
+                                    if (kt < I.n_sink) {
+                                        map = half == 0 ? static_cast<const void*>(&sink_maps.k)
+                                                        : static_cast<const void*>(&sink_maps.v);
+                                    }
+                                }
                                 for (int c = 0; c < Cfg::kChunks; ++c) {
                                     ptx::tma_load_4d(dst + c * kChunkBytes, map, &bars.slot_full[s], c * 64,
-                                                     kt * kTileK, I.hk, I.b);
+                                                     row0, I.hk, I.b);
                                 }
                             }
                             ++issued;
@@ -649,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             k = static_item(n_items, it);
                         }
                         if (k < 0) return false;
-                        In = decode_item(args, k);
+                        In = decode_item<kWin>(args, k);
                         if (In.n_entries > 0) return true;
                     }
                 };
@@ -657,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 int it = -1;
                 Item I;
                 const bool have = next_nonempty(it, I);
-                uint32_t e = have ? kv_entry(args, I, 0) : 0u;
+                uint32_t e = have ? kv_entry<kWin>(args, I, 0) : 0u;
                 if (have) ok = start_item(I, e, 0);
                 for (int j = 0, g = 0; have && ok; ++g) {
                     const int tv = 2 * g + 1;  // V of the current entry
@@ -668,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!last && Cfg::kSepP) {
                         // separate P: the next S MMAs go first (they only wait for the softmax to
                         // have read S), then this tile's P.V MMAs as each P_i arrives
-                        const uint32_t en = kv_entry(args, I, j + 1);
+                        const uint32_t en = kv_entry<kWin>(args, I, j + 1);
                         if (!(ok = wait_full(tk))) break;
                         ptx::tc_fence_after();
                         if ((en & kNeed0) && !(ok = issue_s(0, tk % kSlots))) break;
@@ -681,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         e = en;
                         ++j;
                     } else if (!last) {
-                        const uint32_t en = kv_entry(args, I, j + 1);
+                        const uint32_t en = kv_entry<kWin>(args, I, j + 1);
                         if ((e & kNeed0) && !(ok = issue_pv(0, tv % kSlots))) break;
                         if (!(ok = wait_full(tk))) break;
                         ptx::tc_fence_after();
@@ -702,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (acc[1]) ptx::tc_commit(&bars.o_done[1]);
                         acc[0] = acc[1] = false;
                         if (!next_nonempty(it, I)) break;
-                        e = kv_entry(args, I, 0);
+                        e = kv_entry<kWin>(args, I, 0);
                         j = 0;
                         if (!(ok = start_item(I, e, tk))) break;
                     }
@@ -782,14 +861,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (item < 0) break;
             __syncwarp();  // every lane is done with the previous record
             if (lane == 0) {
-                const Item I = decode_item(args, item);
+                const Item I = decode_item<kWin>(args, item);
                 RowItem r;
                 // reversed walk: entry j is KV tile n_entries - 1 - j, counted from the top tile
                 r.n_entries = args.kv_reverse ? min(args.n_kt, (I.qend1 + kTileK - 1) / kTileK) : I.n_entries;
                 r.pair = I.pair;
                 r.q0 = qtile == 0 ? I.q00 : I.q01;
                 const bool valid = qtile == 0 || I.valid1;
-                if (args.mode == kModeList) {
+                if (kWin) {
+                    r.n_iter = valid ? I.n_entries : 0;
+                } else if (args.mode == kModeList) {
                     r.n_iter = I.n_entries;
                 } else if (!valid) {
                     r.n_iter = 0;
@@ -807,6 +888,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 r.bias_off = (MOD & kModBias) ? static_cast<int64_t>(I.b) * args.bias_s0 +
                                                     static_cast<int64_t>(I.h) * args.bias_s1
                                               : 0;
+                // sliding window: its first key and the sink tiles, in the unused bias offset
+                if constexpr (kWin) r.bias_off = (static_cast<int64_t>(I.n_sink) << 32) | static_cast<uint32_t>(I.win_lo);
                 if (MOD & kModAlibi) {
                     r.slope = args.alibi_generated
                                   ? exp2f(-8.0f * static_cast<float>(I.h + 1) / static_cast<float>(args.heads_q))
@@ -832,8 +915,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!(e & need_bit)) continue;
                 }
                 const int kt = static_cast<int>(e & 0xFFFFu);
-                const int k0 = kt * kTileK;
                 const int q0 = rec->q0;  // loaded ahead of the wait, which hides its latency
+                int k0 = kt * kTileK;
+                bool sink_tile = false;
+                // sliding window, for this warp's 32 rows at positions [wp0, wp0 + 31]: every key
+                // of the tile visible, no key visible, some rows' window starting inside it
+                bool win_full = false, win_none = false, win_low = false;
+                if constexpr (kWin) {
+                    const int64_t span = rec->bias_off;
+                    const int n_sink = static_cast<int>(span >> 32);
+                    sink_tile = kt < n_sink;
+                    k0 = window_tile_start(kt, static_cast<int>(span), n_sink);
+                    const int p0 = args.q_offset + q0;
+                    if (!window_tile_needed(args, k0, sink_tile, p0, args.q_offset + min(args.m, q0 + kTileQ))) continue;
+                    const int wp0 = p0 + wq * 32;
+                    const bool in_sinks = k0 + kTileK <= args.sinks;
+                    win_low = !sink_tile && !in_sinks && k0 <= wp0 + 31 - args.window;
+                    win_full = !win_low && k0 + kTileK - 1 <= wp0 && k0 + kTileK <= (sink_tile ? args.sinks : args.n);
+                    win_none = k0 > wp0 + 31 ||
+                               (!sink_tile && k0 >= args.sinks && k0 + kTileK - 1 <= wp0 - args.window);
+                }
                 // Waits are per thread; the warp re-converges (and agrees) before the
                 // .sync.aligned TMEM accesses that follow.
                 const bool got = ptx::mbar_wait(&bars.s_full[qtile], phases & 1u, abort_flag, args.status,
@@ -843,7 +944,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     break;
                 }
                 ptx::tc_fence_after();
+                if constexpr (kWin && !Cfg::kSepP) {
+                    if (win_none) {  // none of the warp's rows sees a key of the tile
+                        store_zero_p(p_addr);
+                        if (kFarSkip && lane == 0) far_flags[qtile * 4 + wq] = 1;
+                        ptx::mbar_arrive(&bars.p_full[qtile]);
+                        ODF_COUNT(tiles_done);
+                        phases = (phases ^ 1u) | 4u;
+                        continue;
+                    }
+                }
                 const int qi = q0 + row;
+                // the row's position among the keys
+                const int pos = kWin ? args.q_offset + qi : qi;
                 float slope = 0.0f, slope_log2 = 0.0f;
                 if (MOD & kModAlibi) {
                     slope = rec->slope;
@@ -857,8 +970,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // moves only past 2^8, which a sum of at most 2^8 rules out; otherwise S is read
                     // again and the general path below runs (with the same P where the max stays), so
                     // the result is the same as with the max pass first.
-                    const bool interior = k0 + kTileK <= args.n && !(e & bitmap_bit) &&
-                                          !(args.causal && k0 + kTileK - 1 > q0);
+                    const bool interior = kWin ? win_full
+                                               : k0 + kTileK <= args.n && !(e & bitmap_bit) &&
+                                                     !(args.causal && k0 + kTileK - 1 > q0);
                     if (args.scale_log2 > 0.0f && interior && __all_sync(0xffffffffu, m_run != -INFINITY)) {
                         const uint64_t mul2 = ptx::f32x2(args.scale_log2);
                         const uint64_t neg2 = ptx::f32x2(-m_run);
@@ -973,7 +1087,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (MOD & kModSoftcap) {
                     // t = (s * scale + ALiBi) / softcap, with 1/softcap folded into the FMAs that form
                     // it; s[] keeps tanh(t) and the exponent below multiplies by softcap * log2(e)
-                    const float base = static_cast<float>(k0 - qi);
+                    const float base = static_cast<float>(k0 - pos);
                     const uint64_t scale2 = ptx::f32x2(args.scale * args.inv_softcap);
                     const uint64_t slope2 = ptx::f32x2(slope * args.inv_softcap);
                     const uint64_t sb2 = ptx::f32x2(slope * base * args.inv_softcap);
@@ -1035,7 +1149,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 } else if (MOD & kModAlibi) {
                     // s * scale * log2(e) + slope * log2(e) * (base + c) on pairs: base + c (exact for the
                     // integer-valued columns) is stepped in four chains, then one multiply and one FMA
-                    const float base = static_cast<float>(k0 - qi);
+                    const float base = static_cast<float>(k0 - pos);
                     const uint64_t scale2 = ptx::f32x2(args.scale_log2);
                     const uint64_t slope2 = ptx::f32x2(slope_log2);
                     uint64_t col[4];
@@ -1057,10 +1171,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // element mask on boundary tiles (attention.cpp:54-62, 608-617): column c of the
                 // tile survives iff c <= limit (causal kj <= qi, ragged kj < N) and, on tiles that
                 // cover a disallowed BlockMask block, its bit in the row's 128-bit allow mask.
+                if constexpr (kWin) {
+                    if (!win_full) {
+                        // columns [0, limit] that exist and are not ahead of the row (in a sink
+                        // tile: that are sinks), of them those in its window or among the sinks
+                        int limit = min(args.n - 1, pos) - k0;
+                        if (sink_tile) limit = min(limit, args.sinks - 1 - k0);
+                        if (!win_low) {
+#pragma unroll
+                            for (int c = 0; c < 128; ++c) s[c] = (c <= limit) ? s[c] : -INFINITY;
+                        } else {
+                            const int low = pos - args.window + 1 - k0;
+                            const int sk = args.sinks - k0;
+                            uint32_t keep[4];
+#pragma unroll
+                            for (int w = 0; w < 4; ++w)
+                                keep[w] = bits_below(limit + 1 - 32 * w) & (~bits_below(low - 32 * w) | bits_below(sk - 32 * w));
+#pragma unroll
+                            for (int c = 0; c < 128; ++c) s[c] = ((keep[c >> 5] >> (c & 31)) & 1u) ? s[c] : -INFINITY;
+                        }
+                    }
+                }
                 const bool ragged = (k0 + kTileK > args.n);
                 const bool diag = args.causal && (min(args.n, k0 + kTileK) - 1 > q0);
                 const bool bitmap = (e & bitmap_bit) != 0;
-                if (ragged || diag || bitmap) {
+                if (!kWin && (ragged || diag || bitmap)) {
                     int limit = args.n - 1 - k0;
                     if (args.causal) limit = min(limit, qi - k0);
                     if (!bitmap) {  // the tile's entry is the same for the whole warp
@@ -1517,22 +1652,39 @@ CUresult encode_bf16_4d(CUtensorMap* map, const void* ptr, int64_t feat, int64_t
 }
 
 template <int D>
+cudaError_t launch_window(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const SinkMaps<true>& ts,
+                          const FwdArgs& a, int mod, dim3 grid, cudaStream_t stream) {
+    constexpr size_t smem = Config<D>::kSmemBytes;
+    constexpr int W = kModWindow;
+    // d = 128: the plain score always takes the variant that skips the row-max pass of full tiles
+    constexpr int kPlain = D == 128 ? W | kModSkipMax : W;
+    switch (mod) {
+        case 0: flash_fwd_kernel<D, kPlain><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a, ts); break;
+        case 1: flash_fwd_kernel<D, W | 1><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a, ts); break;
+        case 2: flash_fwd_kernel<D, W | 2><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a, ts); break;
+        default: flash_fwd_kernel<D, W | 3><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a, ts); break;
+    }
+    return cudaGetLastError();
+}
+
+template <int D>
 cudaError_t launch_d(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const FwdArgs& a,
                      int mod, dim3 grid, cudaStream_t stream) {
     const size_t smem = Config<D>::kSmemBytes;
+    const SinkMaps<false> none;
     if constexpr (D == 128) {
         if (mod == kModSkipMax) {
-            flash_fwd_kernel<128, kModSkipMax><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a);
+            flash_fwd_kernel<128, kModSkipMax><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a, none);
             return cudaGetLastError();
         }
     }
     switch (mod) {
-        case 0: flash_fwd_kernel<D, 0><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a); break;
-        case 1: flash_fwd_kernel<D, 1><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a); break;
-        case 2: flash_fwd_kernel<D, 2><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a); break;
-        case 3: flash_fwd_kernel<D, 3><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a); break;
-        case 4: flash_fwd_kernel<D, 4><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a); break;
-        default: flash_fwd_kernel<D, 6><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a); break;
+        case 0: flash_fwd_kernel<D, 0><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a, none); break;
+        case 1: flash_fwd_kernel<D, 1><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a, none); break;
+        case 2: flash_fwd_kernel<D, 2><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a, none); break;
+        case 3: flash_fwd_kernel<D, 3><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a, none); break;
+        case 4: flash_fwd_kernel<D, 4><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a, none); break;
+        default: flash_fwd_kernel<D, 6><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a, none); break;
     }
     return cudaGetLastError();
 }
@@ -1644,6 +1796,20 @@ SplitPlan plan_kv_splits(int64_t batch, int64_t heads_q, int64_t seqlen_q, int64
     return sp;
 }
 
+int64_t window_visited_keys(int64_t seqlen_q, int64_t seqlen_k, int64_t window, int64_t sinks) {
+    // a pair's rows see at most window + 255 keys in a run, and the sinks' tiles before it
+    const int64_t run = window < seqlen_k ? window + std::min<int64_t>(seqlen_q, 2 * kTileQ) - 1 : seqlen_k;
+    const int64_t sink_tiles = (std::min(sinks, seqlen_k) + kTileK - 1) / kTileK;
+    // at most one tile more than the keys fill: the sinks' last tile and the run's may both be partial
+    return std::min(run + sink_tiles * kTileK, seqlen_k + (sink_tiles > 0 ? kTileK : 0));
+}
+
+namespace {
+int64_t visited_keys(const FwdArgs& a) {
+    return a.mode == kModeWindow ? window_visited_keys(a.m, a.n, a.window, a.sinks) : a.n;
+}
+}  // namespace
+
 size_t kv_split_bytes(int64_t batch, int64_t heads_q, int64_t seqlen_q, int64_t seqlen_k, int64_t head_dim,
                       bool eligible) {
     const SplitPlan sp = plan_kv_splits(batch, heads_q, seqlen_q, seqlen_k, eligible, kSplitSizingSms);
@@ -1745,6 +1911,14 @@ int setup_device_locked(int device, DeviceState& st, const char** err) {
     if (e == cudaSuccess) e = set_kernel_attrs<128, 4>(&regs_ok);
     if (e == cudaSuccess) e = set_kernel_attrs<128, 6>(&regs_ok);
     if (e == cudaSuccess) e = set_kernel_attrs<128, kModSkipMax>(&regs_ok);
+    if (e == cudaSuccess) e = set_kernel_attrs<64, kModWindow>(&regs_ok);
+    if (e == cudaSuccess) e = set_kernel_attrs<64, kModWindow | 1>(&regs_ok);
+    if (e == cudaSuccess) e = set_kernel_attrs<64, kModWindow | 2>(&regs_ok);
+    if (e == cudaSuccess) e = set_kernel_attrs<64, kModWindow | 3>(&regs_ok);
+    if (e == cudaSuccess) e = set_kernel_attrs<128, kModWindow | kModSkipMax>(&regs_ok);
+    if (e == cudaSuccess) e = set_kernel_attrs<128, kModWindow | 1>(&regs_ok);
+    if (e == cudaSuccess) e = set_kernel_attrs<128, kModWindow | 2>(&regs_ok);
+    if (e == cudaSuccess) e = set_kernel_attrs<128, kModWindow | 3>(&regs_ok);
     if (e == cudaSuccess && !regs_ok) {
         st.status_code = ODF_ERR_UNSUPPORTED;
         *err = "flash kernel built with an unexpected register count (the warp register split needs 168)";
@@ -1841,17 +2015,18 @@ int launch_flash_fwd(FwdLaunch& L, cudaStream_t stream, const char** err) {
     const int64_t n_bh = static_cast<int64_t>(a.batch) * a.heads_q;
     {
         const bool eligible = L.allow_split && a.mode != kModeList && !a.kv_reverse && L.workspace != nullptr;
-        SplitPlan sp = plan_kv_splits(a.batch, a.heads_q, a.m, a.n, eligible, sm_count);
+        SplitPlan sp = plan_kv_splits(a.batch, a.heads_q, a.m, visited_keys(a), eligible, sm_count);
         if (L.forced_splits > 0) sp.n_splits = eligible ? L.forced_splits : 1;
         const size_t room = L.workspace_bytes > kSchedBytes ? L.workspace_bytes - kSchedBytes : 0;
         int64_t splits = sp.n_splits;
         while (splits > 1 && split_partial_bytes(n_bh, a.m, L.head_dim, splits) > room) --splits;
+        const int64_t n_kt = (visited_keys(a) + kTileK - 1) / kTileK;  // KV tiles of an item, at most
         if (splits > 1) {
-            const int64_t per = (a.n_kt + splits - 1) / splits;
-            splits = (a.n_kt + per - 1) / per;
+            const int64_t per = (n_kt + splits - 1) / splits;
+            splits = (n_kt + per - 1) / per;
         }
         if (splits > 1) {
-            const int64_t per = (a.n_kt + splits - 1) / splits;
+            const int64_t per = (n_kt + splits - 1) / splits;
             uint8_t* ws = static_cast<uint8_t*>(L.workspace) + kSchedBytes;
             const int64_t o_plane = n_bh * a.m * L.head_dim;
             a.n_splits = static_cast<int32_t>(splits);
@@ -1869,9 +2044,16 @@ int launch_flash_fwd(FwdLaunch& L, cudaStream_t stream, const char** err) {
     }
 
     CUtensorMap tq, tk, tv;
+    SinkMaps<true> ts;
+    const bool window = a.mode == kModeWindow;
+    // sliding window: keys that no row has reached yet read as zeros
+    const int64_t keys = window ? std::min<int64_t>(a.n, static_cast<int64_t>(a.q_offset) + a.m) : a.n;
+    const int64_t sink_keys = window ? std::max<int64_t>(1, std::min<int64_t>(keys, a.sinks)) : 0;
     if (encode_bf16_4d(&tq, L.q, L.head_dim, a.m, a.heads_q, a.batch, L.q_strides) != CUDA_SUCCESS ||
-        encode_bf16_4d(&tk, L.k, L.head_dim, a.n, a.heads_kv, a.batch, L.k_strides) != CUDA_SUCCESS ||
-        encode_bf16_4d(&tv, L.v, L.head_dim, a.n, a.heads_kv, a.batch, L.v_strides) != CUDA_SUCCESS) {
+        encode_bf16_4d(&tk, L.k, L.head_dim, keys, a.heads_kv, a.batch, L.k_strides) != CUDA_SUCCESS ||
+        encode_bf16_4d(&tv, L.v, L.head_dim, keys, a.heads_kv, a.batch, L.v_strides) != CUDA_SUCCESS ||
+        (window && (encode_bf16_4d(&ts.k, L.k, L.head_dim, sink_keys, a.heads_kv, a.batch, L.k_strides) != CUDA_SUCCESS ||
+                    encode_bf16_4d(&ts.v, L.v, L.head_dim, sink_keys, a.heads_kv, a.batch, L.v_strides) != CUDA_SUCCESS))) {
         *err = "cuTensorMapEncodeTiled rejected a Q/K/V layout (pointers and strides must be 16-byte aligned)";
         return ODF_ERR_INVALID_ARG;
     }
@@ -1888,7 +2070,7 @@ int launch_flash_fwd(FwdLaunch& L, cudaStream_t stream, const char** err) {
         const int64_t kv_unit_bytes = 4 * static_cast<int64_t>(a.n) * L.head_dim;
         int64_t per_block = (int64_t{32} << 20) / (kv_unit_bytes > 0 ? kv_unit_bytes : 1);
         if (per_block < 1) per_block = 1;
-        if (per_block < n_units && a.n_splits == 1 && a.mode != kModeList && L.workspace != nullptr &&
+        if (per_block < n_units && a.n_splits == 1 && a.mode != kModeList && !window && L.workspace != nullptr &&
             L.workspace_bytes >= kSchedBytes && L.head_dim == 128 && !L.has_alibi && !L.has_softcap &&
             !L.has_bias) {  // the instantiation with greedy assignment compiled in
             a.sched = static_cast<unsigned long long*>(L.workspace);
@@ -1961,12 +2143,18 @@ int launch_flash_fwd(FwdLaunch& L, cudaStream_t stream, const char** err) {
     // KV ranges of 16 or more tiles with a plain score: the variant whose unmasked tiles skip the
     // row-max pass (with the row-sum check, N = 4096 measured +2-5%, N = 2048 level; block-masked
     // problems, with few unmasked tiles per row, keep the general variant)
-    if (mod == 0 && L.head_dim == 128 && a.mode != kModeList && a.n_kt >= 16) mod = kModSkipMax;
+    if (mod == 0 && L.head_dim == 128 && a.mode != kModeList && !window && a.n_kt >= 16) mod = kModSkipMax;
     // persistent grid: one CTA per SM (the kernel's shared memory allows one), at most one per item
     const int64_t n_items = static_cast<int64_t>(a.batch) * a.heads_q * a.n_pairs * a.n_splits;
     const dim3 grid(static_cast<unsigned>(n_items < sm_count ? n_items : sm_count), 1, 1);
-    cudaError_t e = (L.head_dim == 64) ? launch_d<64>(tq, tk, tv, a, mod, grid, stream)
-                                       : launch_d<128>(tq, tk, tv, a, mod, grid, stream);
+    cudaError_t e;
+    if (window) {
+        e = (L.head_dim == 64) ? launch_window<64>(tq, tk, tv, ts, a, mod, grid, stream)
+                               : launch_window<128>(tq, tk, tv, ts, a, mod, grid, stream);
+    } else {
+        e = (L.head_dim == 64) ? launch_d<64>(tq, tk, tv, a, mod, grid, stream)
+                               : launch_d<128>(tq, tk, tv, a, mod, grid, stream);
+    }
     if (e == cudaSuccess && a.n_splits > 1) {
         const int64_t rows = n_bh * a.m;
         const unsigned blocks = static_cast<unsigned>((rows + 7) / 8);

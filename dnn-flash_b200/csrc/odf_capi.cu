@@ -343,6 +343,40 @@ size_t odf_fwd_workspace_size(const odf_fwd_params* p) {
     return workspace_with_far_bound(p, p->batch, p->heads_q, p->heads_kv);
 }
 
+int odf_flash_fwd_window_sm100(const odf_fwd_params* p, const odf_window* w, void* stream) {
+    Resolved r;
+    const int rc = validate(p, false, &r);
+    if (rc != ODF_OK) return rc;
+    if (w == nullptr) return fail(ODF_ERR_INVALID_ARG, "window must be non-null");
+    if (w->window < 1 || w->sinks < 0 || w->q_offset < 0)
+        return fail(ODF_ERR_INVALID_ARG, "window must be >= 1, sinks and q_offset >= 0");
+    if (w->q_offset > 0x7fffffffLL - p->seqlen_q - 256 || r.n_kt > 65534)
+        return fail(ODF_ERR_UNSUPPORTED, "positions beyond the kernel's 32 bits");
+    if (p->block_mask != nullptr || p->bias_kind == ODF_BIAS_SAME_SHAPE || p->tile_visits != nullptr)
+        return fail(ODF_ERR_UNSUPPORTED, "a sliding window takes no block mask, bias tensor or tile_visits");
+    if (p->workspace != nullptr && !aligned16(p->workspace))
+        return fail(ODF_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
+    odf::FwdLaunch L = make_launch(p, r);
+    odf::FwdArgs& a = L.args;
+    a.mode = odf::kModeWindow;
+    a.causal = 1;
+    a.kv_reverse = 0;
+    a.q_offset = static_cast<int32_t>(w->q_offset);
+    // a window or sinks past the last position change nothing
+    const int64_t positions = w->q_offset + p->seqlen_q;
+    a.window = static_cast<int32_t>(std::min(w->window, positions));
+    a.sinks = static_cast<int32_t>(std::min(w->sinks, p->seqlen_k));
+    const char* err = "";
+    const int lrc = odf::launch_flash_fwd(L, static_cast<cudaStream_t>(stream), &err);
+    return lrc == ODF_OK ? ODF_OK : fail(lrc, err);
+}
+
+size_t odf_fwd_window_workspace_size(const odf_fwd_params* p, const odf_window* w) {
+    if (p == nullptr || w == nullptr || p->seqlen_q <= 0 || p->seqlen_k <= 0 || w->window < 1 || w->sinks < 0) return 0;
+    const int64_t keys = odf::window_visited_keys(p->seqlen_q, p->seqlen_k, w->window, w->sinks);
+    return odf::kSchedBytes + odf::kv_split_bytes(p->batch, p->heads_q, p->seqlen_q, keys, p->head_dim, true);
+}
+
 int odf_flash_fwd_host(const odf_fwd_params* p) {
     Resolved r;
     int rc = validate(p, true, &r);

@@ -17,6 +17,7 @@ enum TileMode : int32_t {
     kModeDense = 0,   // every KV tile
     kModeCausal = 1,  // KV tiles with kt*128 < min(M, (qt+1)*128)
     kModeList = 2,    // compacted per-query-tile list built from the block mask
+    kModeWindow = 3,  // sliding window and sinks: tiles that start where the pair's window does
 };
 
 // A KV-list entry of a query-tile pair: kv tile index in the low 16 bits, then
@@ -115,6 +116,9 @@ struct FwdArgs {
     // number stall_load (neither the bytes nor the copy), so the MMA warp's wait for that slot runs
     // out and the abort path runs: status word set, roles leave, copies and MMAs drained.
     int32_t stall_load;
+    // kModeWindow: row qi sits at position q_offset + qi of the keys and sees `window` keys up to its
+    // own (clamped to what 32-bit positions need) and the first `sinks` ones.
+    int32_t window, sinks, q_offset;
 };
 
 constexpr uint64_t kDefaultWaitLimitNs = 2000000000ull;
@@ -177,6 +181,8 @@ struct SplitPlan {
 };
 SplitPlan plan_kv_splits(int64_t batch, int64_t heads_q, int64_t seqlen_q, int64_t seqlen_k, bool eligible,
                          int64_t sm_count);
+// Most keys that a pair of query tiles visits in window mode, whole sink tiles counted.
+int64_t window_visited_keys(int64_t seqlen_q, int64_t seqlen_k, int64_t window, int64_t sinks);
 // Optional workspace bytes after kSchedBytes for the fp32 partial O and LSE of that plan (0 without
 // splits), sized for a GPU of kSplitSizingSms SMs.
 constexpr int64_t kSplitSizingSms = 148;

@@ -55,6 +55,10 @@ class FwdParams(C.Structure):
     ]
 
 
+class Window(C.Structure):
+    _fields_ = [("window", C.c_int64), ("sinks", C.c_int64), ("q_offset", C.c_int64)]
+
+
 class PagedCache(C.Structure):
     _fields_ = [
         ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("kv_dtype", C.c_int32),
@@ -111,6 +115,9 @@ def load_library():
     lib.odf_flash_fwd_host.argtypes = [C.POINTER(FwdParams)]
     lib.odf_fwd_workspace_size.argtypes = [C.POINTER(FwdParams)]
     lib.odf_fwd_workspace_size.restype = C.c_size_t
+    lib.odf_flash_fwd_window_sm100.argtypes = [C.POINTER(FwdParams), C.POINTER(Window), C.c_void_p]
+    lib.odf_fwd_window_workspace_size.argtypes = [C.POINTER(FwdParams), C.POINTER(Window)]
+    lib.odf_fwd_window_workspace_size.restype = C.c_size_t
     lib.odf_tile_map_sm100.argtypes = [C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_int64,
                                        C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]
     lib.odf_convert_f32_to_bf16.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
@@ -277,6 +284,56 @@ def flash_fwd(q, k, v, *, causal=False, scale=None, block_mask=None, mask_block=
     # stream they must outlive the launch, so wait for it before releasing them.
     if stream != current and (ws is not None or mask_t is not None):
         torch.cuda.synchronize(dev)
+    del keep
+    return out, (lse if want_lse else None)
+
+
+def flash_fwd_window(q, k, v, *, window, sinks=0, q_offset=0, scale=None, alibi=False, alibi_slopes=None, softcap=0.0,
+                     out_dtype=None, want_lse=True, out=None, lse_out=None, stream=None):
+    """Sliding-window attention with sinks (odf_flash_fwd_window_sm100) on q [B,Hq,M,D], k, v [B,Hkv,N,D] (bf16).
+
+    Row i sits at position p = q_offset + i and sees key j iff j <= p and (p - j < window or j < sinks).
+    ``q_offset``: tokens before this chunk of the prompt (0 for a whole one).  Returns (o, lse) like
+    ``flash_fwd``, asynchronous on ``stream`` (default: torch's current stream).
+    """
+    import torch
+
+    lib = load_library()
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError("q must be [B, Hq, M, D], k and v of one shape [B, Hkv, N, D]")
+    if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+        raise ValueError("q, k and v must be bfloat16")
+    dev = q.device
+    _require_cuda(dev)
+    _on(k, "k", dev)
+    _on(v, "v", dev)
+    B, Hq, M, D = q.shape
+    if alibi_slopes is not None and len(alibi_slopes) != Hq:
+        raise ValueError("alibi_slopes needs one slope per query head")
+    with _launch_on(dev, stream) as handle:
+        if out is None:
+            out = torch.empty((B, Hq, M, D), dtype=out_dtype or torch.float32, device=dev)
+        lse = lse_out
+        if want_lse and lse is None:
+            lse = torch.empty((B, Hq, M), dtype=torch.float32, device=dev)
+        _on(out, "out", dev)
+        _on(lse, "lse_out", dev)
+        if out.shape != q.shape or out.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("out must be float32 or bfloat16 of q's shape")
+        if lse is not None and (lse.shape != (B, Hq, M) or lse.dtype != torch.float32 or not lse.is_contiguous()):
+            raise ValueError("lse_out must be contiguous float32 [B, Hq, M]")
+        p, keep = fill_params(q, k, v, out, lse, causal=True, scale=1.0 / math.sqrt(D) if scale is None else scale,
+                              block_mask=None, mask_block=None, alibi=alibi, alibi_slopes_host=alibi_slopes,
+                              softcap=softcap, workspace=None, visits=None)
+        for field, t, name in ((p.q_strides, q, "q"), (p.k_strides, k, "k"), (p.v_strides, v, "v"), (p.o_strides, out, "out")):
+            for i, s in enumerate(_dense_strides(t, name)):
+                field[i] = s
+        w = Window(window, sinks, q_offset)
+        nbytes = lib.odf_fwd_window_workspace_size(C.byref(p), C.byref(w))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 256 else None
+        if ws is not None:
+            p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
+        _check(lib.odf_flash_fwd_window_sm100(C.byref(p), C.byref(w), handle))
     del keep
     return out, (lse if want_lse else None)
 

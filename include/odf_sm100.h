@@ -113,6 +113,33 @@ int odf_flash_fwd_sm100(const odf_fwd_params* p, void* stream);
    (src/onednn_flash/attention_workspace.cpp:5-20). */
 size_t odf_fwd_workspace_size(const odf_fwd_params* p);
 
+/*
+ * Sliding-window attention with sinks, for prompts and for chunks of them.  Query row i sits at
+ * position p = q_offset + i of the keys and sees key j iff j < seqlen_k, j <= p, and (p - j < window
+ * or j < sinks): the last `window` keys up to its own, and the first `sinks` ones.  A chunk whose
+ * keys are already in K/V passes the number of tokens before it as q_offset; window >= q_offset + M
+ * is causal attention of such a chunk.  ALiBi is slope * (j - p).
+ *
+ * Tensors, score mods, GQA, output and LSE as in odf_fwd_params; p->causal is not read (rows never
+ * see later keys); block masks, bias tensors and tile_visits are refused (ODF_ERR_UNSUPPORTED).
+ * Rows that see nothing get 0 and LSE -inf.  Keys that no row of the call sees may hold anything, NaN
+ * included (evicted pages, room for tokens to come); a non-finite value in a key that some row does see
+ * can reach other rows of its 256-row block.
+ * The token-exact counterpart of the block mask in attention.hpp:20-29, which a window that is
+ * not a multiple of its block size cannot be written as.
+ */
+typedef struct odf_window {
+    int64_t window;    /* >= 1 */
+    int64_t sinks;     /* >= 0 */
+    int64_t q_offset;  /* >= 0; q_offset + seqlen_q below 2^31 */
+} odf_window;
+
+int odf_flash_fwd_window_sm100(const odf_fwd_params* p, const odf_window* w, void* stream);
+
+/* Device scratch bytes for such a call (optional: room for the partial results of KV splits when
+   the launch would leave SMs idle; p->workspace may be NULL). */
+size_t odf_fwd_window_workspace_size(const odf_fwd_params* p, const odf_window* w);
+
 /* Capacity of the library-owned scratch used by odf_flash_fwd_sm100_noalloc. */
 #define ODF_NOALLOC_SCRATCH_BYTES (1u << 20)
 
