@@ -1957,6 +1957,12 @@ int* device_status_ptr(int device) {
     return g_devices[device].status_ptr;
 }
 
+int device_sm_count(int device) {
+    if (device < 0 || device >= kMaxDevices) return 0;
+    std::lock_guard<std::mutex> lock(g_device_mutex);
+    return g_devices[device].sm_count;
+}
+
 int launch_tile_map(int32_t m, int32_t n, int32_t causal, const uint8_t* mask, int32_t mqbs, int32_t mkbs,
                     int32_t mqblocks, int32_t mkblocks, uint8_t* cls_out, cudaStream_t stream) {
     const int n_qt = (m + kTileQ - 1) / kTileQ;

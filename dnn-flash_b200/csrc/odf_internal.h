@@ -169,6 +169,9 @@ void* current_context();
 // Device address of the status word bounded waits write to (current device).
 int* device_status_ptr(int device);
 
+// Its number of SMs (after ensure_device_ready).
+int device_sm_count(int device);
+
 size_t workspace_bytes_for(int64_t seqlen_q, int64_t seqlen_k, bool has_mask);
 
 // KV splits: when a launch's work items (query-tile pairs, or single query tiles) would leave more

@@ -14,13 +14,14 @@ using odf::set_error;
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-int current_device_ready(int** status) {
+int current_device_ready(int** status, int* sm_count) {
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess) return set_error(ODF_ERR_NO_DEVICE, "no CUDA device");
     const char* err = "";
     const int rc = odf::ensure_device_ready(device, &err);
     if (rc != ODF_OK) return set_error(rc, err);
     *status = odf::device_status_ptr(device);
+    *sm_count = odf::device_sm_count(device);
     return ODF_OK;
 }
 
@@ -167,7 +168,8 @@ int odf_paged_decode_sm100(const odf_decode_params* p, void* stream) {
     if (p->workspace == nullptr || p->workspace_bytes < odf_paged_decode_workspace_size(p))
         return set_error(ODF_ERR_INVALID_ARG, "the workspace is smaller than odf_paged_decode_workspace_size() bytes");
     if (!aligned(p->workspace, 16)) return set_error(ODF_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
-    rc = current_device_ready(&a.c.status);
+    int sm_count = 0;
+    rc = current_device_ready(&a.c.status, &sm_count);
     if (rc != ODF_OK) return rc;
     a.q = p->q;
     a.o = p->o;
@@ -193,7 +195,7 @@ int odf_paged_decode_sm100(const odf_decode_params* p, void* stream) {
         }
     }
     a.workspace = p->workspace;
-    a.workspace_bytes = p->workspace_bytes;
+    a.sm_count = sm_count;
     const char* err = "";
     rc = odf::launch_paged_decode(a, static_cast<int32_t>(D), p->cache.kv_dtype, static_cast<cudaStream_t>(stream), &err);
     return rc == ODF_OK ? ODF_OK : set_error(rc, err);
@@ -218,7 +220,8 @@ int odf_paged_append_sm100(const odf_append_params* p, void* stream) {
     rc = resolve(p->k_strides, p->cache.heads_kv, p->tokens, p->cache.head_dim, 2, ks, bad);
     if (rc == ODF_OK) rc = resolve(p->v_strides, p->cache.heads_kv, p->tokens, p->cache.head_dim, 2, vs, bad);
     if (rc != ODF_OK) return rc;
-    rc = current_device_ready(&a.c.status);
+    int sm_count = 0;
+    rc = current_device_ready(&a.c.status, &sm_count);
     if (rc != ODF_OK) return rc;
     a.k = p->k;
     a.v = p->v;
@@ -268,7 +271,8 @@ int odf_page_copy_sm100(const odf_page_copy_params* p, void* stream) {
     }
     if (p->n_pairs == 0) return ODF_OK;
     int* status = nullptr;
-    rc = current_device_ready(&status);
+    int sm_count = 0;
+    rc = current_device_ready(&status, &sm_count);
     if (rc != ODF_OK) return rc;
     odf::CopyArgs a;
     std::memset(&a, 0, sizeof(a));

@@ -41,7 +41,8 @@ struct DecodeArgs {
     int32_t has_alibi, alibi_generated;
     float alibi_slopes[ODF_MAX_EXPLICIT_SLOPES];
     void* workspace;
-    size_t workspace_bytes;
+    int32_t sm_count;
+    int32_t row_tiles, items_per_seq;  // items of one sequence: kv-heads x tiles of 16 query heads
 };
 
 struct AppendArgs {

@@ -7,6 +7,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 #include "paged_internal.h"
 #include "sm100_ptx.cuh"
 
@@ -16,6 +18,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+
+// Decode workspace: a counter per CTA, then two partial results per CTA.
+constexpr size_t kDecodeCounterBytes = 2048;
 
 __device__ __forceinline__ void bad_page(const PagedView& c) {
     if (c.status) atomicCAS(c.status, 0, ODF_ERR_BAD_PAGE);
@@ -57,90 +62,626 @@ __device__ __forceinline__ bool row_offsets(const PagedView& c, const int32_t* t
     return true;
 }
 
-template <int V>
-__device__ __forceinline__ void load_row(const uint8_t* p, int lane, bool e4m3, float* x) {
-    if (e4m3) {
-        const __nv_fp8_e4m3* s = reinterpret_cast<const __nv_fp8_e4m3*>(p) + lane * V;
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = static_cast<float>(s[i]);
-    } else {
-        const __nv_bfloat16* s = reinterpret_cast<const __nv_bfloat16*>(p) + lane * V;
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = __bfloat162float(s[i]);
-    }
+// ------------------------------------------------------------------------------ decode attention
+//
+// What bounds it is the cache: every visible key and value is read once (2 d e bytes a key and
+// kv-head) against 4 d FLOP per query head, at most a few dozen FLOP a byte, so the kernel is built
+// around keeping loads in flight and the arithmetic behind them is one m16n8k16 product per 16
+// keys (S = Q K^T, then O += P V, the query heads of one kv-head as the 16 rows).  tcgen05 would
+// want 128 rows; there are at most 16, and the warp-level product keeps up (at d = 128 a key costs two
+// of them, against 22 clocks that its 512 bytes take at the SM's share of HBM).
+//
+// Work: an item is (sequence, kv-head, 16 query heads); its visible keys are cut into slices of 16.  The slices
+// of all items in a row are dealt to the CTAs in equal consecutive runs, whatever the lengths, by a
+// prefix sum over the lengths that every CTA does for itself.  A run holds pieces of one or
+// several items; an item that lies in one run is written out directly, the pieces of one that
+// does not go to the workspace as fp32 O, max and sum, and the CTA that is last to finish (a
+// counter that wraps to zero) joins them in order, so the result does not depend on who that is.
+//
+// Inside a piece the warps take slices in turn, each with a softmax of its own (running max and sum,
+// O in registers) and a ring of its own in shared memory, filled by cp.async kStages - 1 slices
+// ahead, across piece borders: no barrier between warps until a piece ends and their parts are joined.
+constexpr int kDecodeWarps = 4;
+constexpr int kDecodeThreads = kDecodeWarps * 32;
+constexpr int kDecodeMaxCtas = 2 * 148;  // two per SM
+constexpr int kSlice = 16;               // keys
+constexpr int kRowsMax = 16;             // query heads of an item
+constexpr int kMinSlices = 16;           // fewest slices worth a CTA of their own
+constexpr int kMergeCols = 32;           // columns of O joined at a time
+constexpr int kMergeStride = kMergeCols + 8;  // floats: 8 banks from row to row
+
+template <int D, bool kE4M3>
+struct DecodeCfg {
+    static constexpr int kRowBytes = D * (kE4M3 ? 1 : 2);
+    static constexpr int kTileBytes = kSlice * kRowBytes;   // K or V of a slice
+    static constexpr int kStageBytes = 2 * kTileBytes;
+    // 24 KB a warp: with two CTAs of four warps, 128 KB of loads in flight on the SM behind the
+    // slice that is being computed
+    static constexpr int kStages = kStageBytes >= 8192 ? 3 : kStageBytes >= 4096 ? 6 : 8;
+    static constexpr int kChunks = kRowBytes / 16;          // 16-byte chunks of a row
+    static constexpr int kOffMerge = kDecodeWarps * kStages * kStageBytes;
+    static constexpr int kOffStats = kOffMerge + kDecodeWarps * kRowsMax * kMergeStride * 4;
+    static constexpr int kOffMask = kOffStats + 2 * kDecodeWarps * kRowsMax * 4;
+    static constexpr int kOffPlan = kOffMask + kDecodeWarps * kStages * 4;
+    static constexpr int kSmemBytes = kOffPlan + 64 + kDecodeWarps * 8;
+    static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
+};
+
+// Chunk c of row r lies at chunk c ^ swizzle(r): eight consecutive rows then hold one chunk index in
+// different banks.
+template <int D, bool kE4M3>
+__device__ __forceinline__ int swizzle(int r) {
+    if constexpr (DecodeCfg<D, kE4M3>::kChunks == 4) return (r >> 1) & 3;
+    return r & 7;
 }
 
-// One block per (batch, q-head), a key per warp at a time.
-constexpr int kDecodeWarps = 4;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+// D[16 x 8] += A[16 x 16] B[16 x 8], fp32 sums, bf16 or f16 operands.
+template <bool kHalf>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (kHalf)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four e4m3 values as two pairs of f16 (exact).
+__device__ __forceinline__ void e4m3x4_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
 
-template <int D>
-__global__ void __launch_bounds__(kDecodeWarps * 32) paged_decode_kernel(const __grid_constant__ DecodeArgs a, bool e4m3) {
-    constexpr int V = D / 32;
-    const int b = blockIdx.x / a.heads_q;
-    const int h = blockIdx.x - b * a.heads_q;
-    const int hk = h / a.group;
+__host__ __device__ constexpr int64_t run_start(int64_t cta, int64_t total, int64_t ctas) { return cta * total / ctas; }
+// The CTA whose run holds slice s.
+__device__ __forceinline__ int run_owner(int64_t s, int64_t total, int64_t ctas) {
+    return static_cast<int>(((s + 1) * ctas - 1) / total);
+}
+
+// Walks a CTA's run piece by piece: slices [s0, s1) of item r of sequence b.
+struct RunCursor {
+    int b, r, s0, s1;
+    int64_t left;  // slices of the run after this piece
+    Visible vis;
+    int n;         // slices of the item
+    __device__ __forceinline__ void enter(const DecodeArgs& a) {
+        vis = visible_keys(a, __ldg(a.lens + b));
+        n = max(1, (vis.count + kSlice - 1) / kSlice);
+    }
+    __device__ __forceinline__ void cut() {
+        s1 = static_cast<int>(min(static_cast<int64_t>(n), s0 + left));
+        left -= s1 - s0;
+    }
+    __device__ __forceinline__ bool next(const DecodeArgs& a) {
+        if (left <= 0) return false;
+        s0 = 0;
+        if (++r == a.items_per_seq) {
+            r = 0;
+            ++b;
+            enter(a);
+        }
+        cut();
+        return true;
+    }
+};
+
+template <int D, bool kE4M3>
+__global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const __grid_constant__ DecodeArgs a) {
+    using Cfg = DecodeCfg<D, kE4M3>;
+    constexpr int kStages = Cfg::kStages;
+    constexpr int kSteps = D / 16;   // products of S per 8 keys
+    constexpr int kBlocks = D / 8;   // column blocks of O
+    // 8-bit path: weights as f16 times 2^15, which keeps 11 bits of every weight down to 2^-29 of the
+    // row's largest (and something down to 2^-39)
+    constexpr float kShift = kE4M3 ? 15.0f : 0.0f;
+    extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Visible vis = visible_keys(a, __ldg(a.lens + b));
-    const int32_t* table = a.c.table + b * a.c.table_stride;
-    const float ks = a.c.k_scale ? a.c.k_scale[hk] : 1.0f;
-    const float vs = a.c.v_scale ? a.c.v_scale[hk] : 1.0f;
-    float slope = 0.0f;
-    if (a.has_alibi)
-        slope = a.alibi_generated ? exp2f(-8.0f * static_cast<float>(h + 1) / static_cast<float>(a.heads_q)) : a.alibi_slopes[h];
-    float q[V], acc[V];
-    load_row<V>(reinterpret_cast<const uint8_t*>(static_cast<const __nv_bfloat16*>(a.q) + b * a.q_b + h * a.q_h), lane, false, q);
+    const int g = lane >> 2, t = lane & 3;
+    float* merge = reinterpret_cast<float*>(smem + Cfg::kOffMerge);
+    float* stat_m = reinterpret_cast<float*>(smem + Cfg::kOffStats);
+    float* stat_l = stat_m + kDecodeWarps * kRowsMax;
+    uint32_t* masks = reinterpret_cast<uint32_t*>(smem + Cfg::kOffMask) + warp * kStages;
+
+    // ---- the run of this CTA
+    RunCursor cur;
+    int64_t total, first;
+    int ctas;
+    {
+        int64_t* plan = reinterpret_cast<int64_t*>(smem + Cfg::kOffPlan);
+        int64_t* wsum = plan + 8;
+        const int per = (a.batch + kDecodeThreads - 1) / kDecodeThreads;
+        const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
+        int64_t mine = 0;
+        for (int b = b0; b < b1; ++b) {
+            const Visible v = visible_keys(a, __ldg(a.lens + b));
+            mine += max(1, (v.count + kSlice - 1) / kSlice);
+        }
+        mine *= a.items_per_seq;
+        int64_t incl = mine;
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    for (int u = warp; u < vis.count; u += kDecodeWarps) {
-        const int j = vis.key(u);
-        int64_t ko, vo;
-        if (!row_offsets(a.c, table, j, hk, &ko, &vo)) continue;
-        float k[V], v[V];
-        load_row<V>(a.c.k + ko, lane, e4m3, k);
-        load_row<V>(a.c.v + vo, lane, e4m3, v);
-        float s = 0.0f;
+        for (int off = 1; off < 32; off <<= 1) {
+            const int64_t o = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += o;
+        }
+        if (lane == 31) wsum[warp] = incl;
+        __syncthreads();
+        total = 0;
+        int64_t before = incl - mine;
 #pragma unroll
-        for (int i = 0; i < V; ++i) s = fmaf(q[i], k[i], s);
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        s = s * (a.scale * ks) + slope * static_cast<float>(j - (vis.len - 1));
-        if (a.softcap > 0.0f) s = a.softcap * tanhf(s * a.inv_softcap);
-        const float mn = fmaxf(m, s);
-        const float alpha = m == -INFINITY ? 0.0f : expf(m - mn);
-        const float p = expf(s - mn);
-        l = l * alpha + p;
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = acc[i] * alpha + p * v[i];
-        m = mn;
+        for (int w = 0; w < kDecodeWarps; ++w) {
+            if (w < warp) before += wsum[w];
+            total += wsum[w];
+        }
+        const int64_t worth = (total + kMinSlices - 1) / kMinSlices;
+        ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), worth));
+        if (static_cast<int>(blockIdx.x) >= ctas) return;
+        first = run_start(blockIdx.x, total, ctas);
+        if (mine > 0 && first >= before && first < before + mine) {
+            int64_t at = before;
+            for (int b = b0;; ++b) {
+                const Visible v = visible_keys(a, __ldg(a.lens + b));
+                const int n = max(1, (v.count + kSlice - 1) / kSlice);
+                const int64_t all = static_cast<int64_t>(n) * a.items_per_seq;
+                if (first < at + all) {
+                    plan[0] = b;
+                    plan[1] = (first - at) / n;
+                    plan[2] = (first - at) % n;
+                    break;
+                }
+                at += all;
+            }
+        }
+        __syncthreads();
+        cur.b = static_cast<int>(plan[0]);
+        cur.r = static_cast<int>(plan[1]);
+        cur.s0 = static_cast<int>(plan[2]);
+        cur.left = run_start(blockIdx.x + 1, total, ctas) - first;
+        cur.enter(a);
+        cur.cut();
     }
-    __shared__ float sm[kDecodeWarps], sl[kDecodeWarps], so[kDecodeWarps][D];
-    if (lane == 0) {
-        sm[warp] = m;
-        sl[warp] = l;
-    }
+
+    // ---- loads: this warp's slices s0 + warp, s0 + warp + 4, ... of every piece, in order
+    const uint32_t ring = ptx::smem_u32(smem) + warp * (kStages * Cfg::kStageBytes);
+    RunCursor ld = cur;
+    int ld_s = ld.s0 + warp;
+    bool ld_more = true;
+    int ld_slot = 0;  // ring slot of the next load
+    int ld_page = 0, ld_in_page = 0;
+    bool ld_key = false;
+    // finds the next slice and asks for its page ids: lanes 0-15 stand for its keys' K rows, 16-31
+    // for their V rows
+    auto seek = [&]() {
+        while (ld_s >= ld.s1) {
+            if (!ld.next(a)) {
+                ld_more = false;
+                return;
+            }
+            ld_s = ld.s0 + warp;
+        }
+        const int u = ld_s * kSlice + (lane & 15);
+        ld_key = u < ld.vis.count;
+        if (ld_key) {
+            const int j = ld.vis.key(u);
+            const int at = static_cast<int>(fast_div(static_cast<uint32_t>(j), a.c.fd_page));
+            ld_in_page = j - at * a.c.page_size;
+            ld_page = __ldg(a.c.table + ld.b * a.c.table_stride + at);
+        }
+    };
+    auto load = [&]() {
+        if (ld_more) {
+            const int hk = ld.r / a.row_tiles;
+            int64_t off = -1;
+            if (ld_key) {
+                if (ld_page < 0 || ld_page >= a.c.num_pages)
+                    bad_page(a.c);
+                else if (lane < 16)
+                    off = ld_page * a.c.k_page + hk * a.c.k_head + ld_in_page * a.c.k_slot;
+                else
+                    off = ld_page * a.c.v_page + hk * a.c.v_head + ld_in_page * a.c.v_slot;
+            }
+            const uint32_t seen = __ballot_sync(0xffffffffu, off >= 0);
+            if (lane == 0) masks[ld_slot] = seen & 0xffffu;
+            constexpr int kRowsPer = 32 / Cfg::kChunks;  // rows per instruction
+            const int c = lane % Cfg::kChunks;
+            const uint32_t dst = ring + ld_slot * Cfg::kStageBytes;
 #pragma unroll
-    for (int i = 0; i < V; ++i) so[warp][lane * V + i] = acc[i];
-    __syncthreads();
-    float mx = -INFINITY, sum = 0.0f;
-    for (int w = 0; w < kDecodeWarps; ++w) mx = fmaxf(mx, sm[w]);
-    float wt[kDecodeWarps];
-    for (int w = 0; w < kDecodeWarps; ++w) {
-        wt[w] = sl[w] == 0.0f ? 0.0f : expf(sm[w] - mx);
-        sum += wt[w] * sl[w];
+            for (int i = 0; i < kSlice / kRowsPer; ++i) {
+                const int row = i * kRowsPer + lane / Cfg::kChunks;
+                const uint32_t at = dst + row * Cfg::kRowBytes + ((c ^ swizzle<D, kE4M3>(row)) << 4);
+                const int64_t ko = __shfl_sync(0xffffffffu, off, row);
+                const int64_t vo = __shfl_sync(0xffffffffu, off, 16 + row);
+                // rows that are not seen read as zeros (their bytes are not touched)
+                cp_async16(at, a.c.k + (ko < 0 ? 0 : ko + c * 16), ko < 0 ? 0 : 16);
+                cp_async16(at + Cfg::kTileBytes, a.c.v + (vo < 0 ? 0 : vo + c * 16), vo < 0 ? 0 : 16);
+            }
+            ld_slot = ld_slot + 1 == kStages ? 0 : ld_slot + 1;
+            ld_s += kDecodeWarps;
+            seek();
+        }
+        cp_async_commit();  // an empty group when there is nothing left, so that the count below holds
+    };
+    seek();
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) load();
+
+    int slot = 0;  // ring slot of the next slice to compute
+    int64_t item0 = first - cur.s0;  // slice number, over all items, of the item's first
+    for (;;) {
+        const int hk = cur.r / a.row_tiles;
+        const int row0 = (cur.r - hk * a.row_tiles) * kRowsMax;  // first query head of the item, within the group
+        const int rows = min(kRowsMax, a.group - row0);
+        const int h0 = hk * a.group + row0;
+
+        // ---- Q as the A operand of S = Q K^T: rows g and g + 8
+        uint32_t qf[kSteps][4];
+        float unit[2] = {1.0f, 1.0f};  // 8-bit path: what one unit of S is worth, by row
+        {
+            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + cur.b * a.q_b + h0 * a.q_h;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int row = g + 8 * hf;
+                const bool ok = row < rows;
+                const __nv_bfloat16* qr = q + (ok ? row : 0) * a.q_h;
+                if constexpr (!kE4M3) {
+#pragma unroll
+                    for (int kk = 0; kk < kSteps; ++kk) {
+                        qf[kk][hf] = ok ? __ldg(reinterpret_cast<const uint32_t*>(qr + kk * 16 + 2 * t)) : 0u;
+                        qf[kk][2 + hf] = ok ? __ldg(reinterpret_cast<const uint32_t*>(qr + kk * 16 + 8 + 2 * t)) : 0u;
+                    }
+                } else {
+                    // lane t holds the D/4 consecutive features whose 8-bit keys it reads; as f16, scaled
+                    // by a power of two that puts the row's largest at 2^14 (exact down to 2^-30 of it)
+                    uint2 w[kSteps];
+                    float mx = 0.0f;
+#pragma unroll
+                    for (int kk = 0; kk < kSteps; ++kk) {
+                        w[kk] = ok ? __ldg(reinterpret_cast<const uint2*>(qr + (D / 4) * t + 4 * kk)) : make_uint2(0u, 0u);
+                        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(__uint_as_float(w[kk].x << 16)), fabsf(__uint_as_float(w[kk].x & 0xFFFF0000u))),
+                                             fmaxf(fabsf(__uint_as_float(w[kk].y << 16)), fabsf(__uint_as_float(w[kk].y & 0xFFFF0000u)))));
+                    }
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    // exponent of the largest, kept where 2^(14 - e) and its inverse are normal
+                    int e = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
+                    e = mx == 0.0f || e > 127 ? 14 : max(e, -100);
+                    const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
+                    unit[hf] = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+#pragma unroll
+                    for (int kk = 0; kk < kSteps; ++kk) {
+                        qf[kk][hf] = pack_half2(__uint_as_float(w[kk].x << 16) * up, __uint_as_float(w[kk].x & 0xFFFF0000u) * up);
+                        qf[kk][2 + hf] = pack_half2(__uint_as_float(w[kk].y << 16) * up, __uint_as_float(w[kk].y & 0xFFFF0000u) * up);
+                    }
+                }
+            }
+        }
+        float slope[2] = {0.0f, 0.0f};
+        if (a.has_alibi) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int h = h0 + g + 8 * hf;
+                if (g + 8 * hf < rows)
+                    slope[hf] = a.alibi_generated ? exp2f(-8.0f * static_cast<float>(h + 1) / static_cast<float>(a.heads_q))
+                                                  : a.alibi_slopes[h];
+            }
+        }
+        const float ks = a.c.k_scale ? __ldg(a.c.k_scale + hk) : 1.0f;
+        const bool capped = a.softcap > 0.0f;
+        // score = S * mul + slope * (j - p): log2 units, or units of the soft-cap
+        const float into = capped ? a.inv_softcap : kLog2e;
+        float mul[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            mul[hf] = a.scale * unit[hf] * ks * into;
+            slope[hf] *= into;
+        }
+
+        float o[kBlocks][4];
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+        for (int s = cur.s0 + warp; s < cur.s1; s += kDecodeWarps) {
+            cp_async_wait<kStages - 2>();
+            __syncwarp();
+            load();  // into the slot whose slice every lane has finished
+            const uint32_t kt = ring + slot * Cfg::kStageBytes;
+            const uint32_t vt = kt + Cfg::kTileBytes;
+            const uint32_t seen = masks[slot];
+            slot = slot + 1 == kStages ? 0 : slot + 1;
+
+            // S[16 rows x 16 keys]: keys 2t, 2t + 1 of the lower and the upper eight
+            float sc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+            if constexpr (!kE4M3) {
+                const int key = ((lane >> 4) << 3) + (lane & 7);
+                const uint32_t at = kt + key * Cfg::kRowBytes + ((((lane >> 3) & 1) ^ swizzle<D, kE4M3>(key)) << 4);
+#pragma unroll
+                for (int kk = 0; kk < kSteps; ++kk) {
+                    uint32_t b[4];
+                    ldmatrix4(at ^ (kk << 5), b);
+                    mma16816<false>(sc[0], qf[kk], b[0], b[1]);
+                    mma16816<false>(sc[1], qf[kk], b[2], b[3]);
+                }
+            } else {
+#pragma unroll
+                for (int nb = 0; nb < 2; ++nb) {
+                    const int key = nb * 8 + g;
+#pragma unroll
+                    for (int c = 0; c < kSteps / 4; ++c) {
+                        const int chunk = (kSteps / 4) * t + c;
+                        const uint4 w = lds128(kt + key * Cfg::kRowBytes + ((chunk ^ swizzle<D, kE4M3>(key)) << 4));
+                        uint32_t b0, b1;
+                        e4m3x4_to_half(w.x, b0, b1);
+                        mma16816<true>(sc[nb], qf[4 * c + 0], b0, b1);
+                        e4m3x4_to_half(w.y, b0, b1);
+                        mma16816<true>(sc[nb], qf[4 * c + 1], b0, b1);
+                        e4m3x4_to_half(w.z, b0, b1);
+                        mma16816<true>(sc[nb], qf[4 * c + 2], b0, b1);
+                        e4m3x4_to_half(w.w, b0, b1);
+                        mma16816<true>(sc[nb], qf[4 * c + 3], b0, b1);
+                    }
+                }
+            }
+
+            // score mods, mask, running max
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = nb * 8 + 2 * t + (i & 1);
+                    float x = sc[nb][i] * mul[i >> 1];
+                    if (a.has_alibi)
+                        x += slope[i >> 1] * static_cast<float>(cur.vis.key(s * kSlice + key) - (cur.vis.len - 1));
+                    if (capped) x = a.softcap * kLog2e * tanhf(x);
+                    x = (seen >> key) & 1u ? x : -INFINITY;
+                    sc[nb][i] = x;
+                    mx[i >> 1] = fmaxf(mx[i >> 1], x);
+                }
+            }
+            bool moved = false;
+            float alpha[2];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
+                mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
+                const float mn = fmaxf(m[hf], mx[hf]);
+                alpha[hf] = mn > m[hf] ? ptx::ex2(m[hf] - mn) : 1.0f;
+                moved |= mn > m[hf];
+                m[hf] = mn;
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+                l[0] *= alpha[0];
+                l[1] *= alpha[1];
+#pragma unroll
+                for (int j = 0; j < kBlocks; ++j) {
+                    o[j][0] *= alpha[0];
+                    o[j][1] *= alpha[0];
+                    o[j][2] *= alpha[1];
+                    o[j][3] *= alpha[1];
+                }
+            }
+            const float ref[2] = {(m[0] == -INFINITY ? 0.0f : m[0]) - kShift, (m[1] == -INFINITY ? 0.0f : m[1]) - kShift};
+            // P in the operand's type; l sums it before that rounding
+            uint32_t p[4];
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb) {
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[i] = ptx::ex2(sc[nb][i] - ref[i >> 1]);
+                l[0] += e[0] + e[1];
+                l[1] += e[2] + e[3];
+                p[2 * nb] = kE4M3 ? pack_half2(e[0], e[1]) : ptx::pack_bf16x2(e[0], e[1]);
+                p[2 * nb + 1] = kE4M3 ? pack_half2(e[2], e[3]) : ptx::pack_bf16x2(e[2], e[3]);
+            }
+
+            // O += P V
+            if constexpr (!kE4M3) {
+                const int key = (((lane >> 3) & 1) << 3) + (lane & 7);
+                const uint32_t at = vt + key * Cfg::kRowBytes + (((lane >> 4) ^ swizzle<D, kE4M3>(key)) << 4);
+#pragma unroll
+                for (int dd = 0; dd < kSteps; ++dd) {
+                    uint32_t b[4];
+                    ldmatrix4_trans(at ^ (dd << 5), b);
+                    mma16816<false>(o[2 * dd], p, b[0], b[1]);
+                    mma16816<false>(o[2 * dd + 1], p, b[2], b[3]);
+                }
+            } else {
+                // column n of block j is feature (D/8) n + j: lane g reads D/8 consecutive features of
+                // keys 2t, 2t+1, 2t+8, 2t+9 and pairs the keys' bytes feature by feature
+                uint32_t w[4][D / 32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = 2 * t + (i & 1) + 8 * (i >> 1);
+                    if constexpr (D == 128) {
+                        const uint4 x = lds128(vt + key * Cfg::kRowBytes + ((g ^ swizzle<D, kE4M3>(key)) << 4));
+                        w[i][0] = x.x;
+                        w[i][1] = x.y;
+                        w[i][2] = x.z;
+                        w[i][3] = x.w;
+                    } else {
+                        const uint2 x = lds64(vt + key * Cfg::kRowBytes + (((g >> 1) ^ swizzle<D, kE4M3>(key)) << 4) + (g & 1) * 8);
+                        w[i][0] = x.x;
+                        w[i][1] = x.y;
+                    }
+                }
+#pragma unroll
+                for (int q4 = 0; q4 < D / 32; ++q4) {
+                    uint32_t b0[4], b1[4];
+                    e4m3x4_to_half(__byte_perm(w[0][q4], w[1][q4], 0x5140), b0[0], b0[1]);
+                    e4m3x4_to_half(__byte_perm(w[0][q4], w[1][q4], 0x7362), b0[2], b0[3]);
+                    e4m3x4_to_half(__byte_perm(w[2][q4], w[3][q4], 0x5140), b1[0], b1[1]);
+                    e4m3x4_to_half(__byte_perm(w[2][q4], w[3][q4], 0x7362), b1[2], b1[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mma16816<true>(o[4 * q4 + i], p, b0[i], b1[i]);
+                }
+            }
+        }
+
+        // ---- the warps' parts of the piece: a common max, then O in strips of kMergeCols columns
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
+            l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+            if (t == 0) {
+                stat_m[warp * kRowsMax + g + 8 * hf] = m[hf];
+                stat_l[warp * kRowsMax + g + 8 * hf] = l[hf];
+            }
+        }
+        __syncthreads();
+        const int row = threadIdx.x >> 3;  // of the joined result: 16 rows x 8 threads of 4 columns
+        const bool row_ok = row < rows;
+        float M = -INFINITY, L = 0.0f, wt[kDecodeWarps];
+#pragma unroll
+        for (int w = 0; w < kDecodeWarps; ++w) M = fmaxf(M, stat_m[w * kRowsMax + row]);
+#pragma unroll
+        for (int w = 0; w < kDecodeWarps; ++w) {
+            const float mw = stat_m[w * kRowsMax + row];
+            wt[w] = mw == -INFINITY ? 0.0f : ptx::ex2(mw - M);
+            L += wt[w] * stat_l[w * kRowsMax + row];
+        }
+        const bool whole = cur.s0 == 0 && cur.s1 == cur.n;
+        // partial results: slot 2c + 1 for the item that starts in this run, 2c for one that started before
+        float* slots = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + kDecodeCounterBytes);
+        constexpr int kSlotFloats = kRowsMax * D + 2 * kRowsMax;
+        float* part = slots + (2 * static_cast<int64_t>(blockIdx.x) + (cur.s0 == 0 ? 1 : 0)) * kSlotFloats;
+        const float vs = a.c.v_scale ? __ldg(a.c.v_scale + hk) : 1.0f;
+        auto write_out = [&](int r, int col, float4 x, float sum) {
+            const float inv = sum == 0.0f ? 0.0f : vs / sum;  // a row that sees no key: 0
+            x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+            const int64_t at = cur.b * a.o_b + (h0 + r) * a.o_h + col;
+            if (a.o_bf16)
+                *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.o) + at) =
+                    make_uint2(ptx::pack_bf16x2(x.x, x.y), ptx::pack_bf16x2(x.z, x.w));
+            else
+                *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at) = x;
+        };
+        auto write_lse = [&](int r, float mr, float sum) {
+            if (a.lse)
+                a.lse[static_cast<int64_t>(cur.b) * a.heads_q + h0 + r] =
+                    sum == 0.0f ? -INFINITY : (mr + (log2f(sum) - kShift)) * kLn2;
+        };
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += kMergeCols) {
+#pragma unroll
+            for (int j = 0; j < kBlocks; ++j) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = g + 8 * (i >> 1);
+                    const int d = kE4M3 ? (D / 8) * (2 * t + (i & 1)) + j : 8 * j + 2 * t + (i & 1);
+                    if (r < rows && d >= c0 && d < c0 + kMergeCols)
+                        merge[(warp * kRowsMax + r) * kMergeStride + d - c0] = o[j][i];
+                }
+            }
+            __syncthreads();
+            if (row_ok) {
+                const int col = (threadIdx.x & 7) * 4;
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < kDecodeWarps; ++w) {
+                    const float4 y = *reinterpret_cast<const float4*>(merge + (w * kRowsMax + row) * kMergeStride + col);
+                    x.x += wt[w] * y.x;
+                    x.y += wt[w] * y.y;
+                    x.z += wt[w] * y.z;
+                    x.w += wt[w] * y.w;
+                }
+                if (whole)
+                    write_out(row, c0 + col, x, L);
+                else
+                    *reinterpret_cast<float4*>(part + row * D + c0 + col) = x;
+            }
+            __syncthreads();
+        }
+        if (row_ok && (threadIdx.x & 7) == 0) {
+            if (whole) {
+                write_lse(row, M, L);
+            } else {
+                part[kRowsMax * D + row] = M;
+                part[kRowsMax * D + kRowsMax + row] = L;
+            }
+        }
+        if (!whole) {
+            const int c_first = run_owner(item0, total, ctas);
+            const int pieces = run_owner(item0 + cur.n - 1, total, ctas) - c_first + 1;
+            __threadfence();
+            __syncthreads();
+            int* last = reinterpret_cast<int*>(stat_m);
+            if (threadIdx.x == 0) {
+                const unsigned int old =
+                    atomicInc(static_cast<unsigned int*>(a.workspace) + c_first, static_cast<unsigned int>(pieces - 1));
+                *last = old == static_cast<unsigned int>(pieces - 1);
+            }
+            __syncthreads();
+            const bool join = *last != 0;
+            __syncthreads();
+            if (join && row_ok) {
+                __threadfence();
+                const float* p0 = slots + (2 * static_cast<int64_t>(c_first) + 1) * kSlotFloats;  // the first piece
+                auto piece = [&](int k) { return k == 0 ? p0 : slots + 2 * static_cast<int64_t>(c_first + k) * kSlotFloats; };
+                float mj = -INFINITY, lj = 0.0f;
+                for (int k = 0; k < pieces; ++k) mj = fmaxf(mj, __ldcg(piece(k) + kRowsMax * D + row));
+                float4 x[D / 32];
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int k = 0; k < pieces; ++k) {
+                    const float* pk = piece(k);
+                    const float mk = __ldcg(pk + kRowsMax * D + row);
+                    const float w = mk == -INFINITY ? 0.0f : ptx::ex2(mk - mj);
+                    lj += w * __ldcg(pk + kRowsMax * D + kRowsMax + row);
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(pk + row * D + i * 32) + (threadIdx.x & 7));
+                        x[i].x += w * y.x;
+                        x[i].y += w * y.y;
+                        x[i].z += w * y.z;
+                        x[i].w += w * y.w;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) write_out(row, i * 32 + (threadIdx.x & 7) * 4, x[i], lj);
+                if ((threadIdx.x & 7) == 0) write_lse(row, mj, lj);
+            }
+        }
+        item0 += cur.n;
+        if (!cur.next(a)) break;
     }
-    if (threadIdx.x < D) {
-        float o = 0.0f;
-        for (int w = 0; w < kDecodeWarps; ++w)
-            if (sl[w] != 0.0f) o += wt[w] * so[w][threadIdx.x];
-        o = vis.count > 0 ? o / sum * vs : 0.0f;
-        const int64_t at = b * a.o_b + h * a.o_h + threadIdx.x;
-        if (a.o_bf16)
-            static_cast<__nv_bfloat16*>(a.o)[at] = __float2bfloat16_rn(o);
-        else
-            static_cast<float*>(a.o)[at] = o;
-    }
-    if (threadIdx.x == 0 && a.lse) a.lse[static_cast<int64_t>(b) * a.heads_q + h] = vis.count > 0 ? mx + logf(sum) : -INFINITY;
+    cp_async_wait<0>();
 }
 
 // A thread per 16 bytes of new row: K, then V.
@@ -237,16 +778,41 @@ cudaError_t launch_copy(const CopyArgs& a, int64_t first, int64_t count, cudaStr
 
 }  // namespace
 
-size_t decode_workspace_bytes(int32_t) { return 256; }
+size_t decode_workspace_bytes(int32_t head_dim) {
+    return kDecodeCounterBytes + 2 * sizeof(float) * kDecodeMaxCtas * (static_cast<size_t>(kRowsMax) * head_dim + 2 * kRowsMax);
+}
+
+namespace {
+
+template <int D, bool kE4M3>
+cudaError_t launch_decode(const DecodeArgs& a, unsigned grid, cudaStream_t stream) {
+    constexpr int smem = DecodeCfg<D, kE4M3>::kSmemBytes;
+    const cudaError_t e =
+        cudaFuncSetAttribute(paged_decode_kernel<D, kE4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    paged_decode_kernel<D, kE4M3><<<grid, kDecodeThreads, smem, stream>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace
 
 int launch_paged_decode(DecodeArgs& a, int32_t head_dim, int32_t kv_dtype, cudaStream_t stream, const char** err) {
-    const unsigned grid = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.heads_q);
-    const bool e4m3 = kv_dtype == ODF_DTYPE_E4M3;
-    if (head_dim == 64)
-        paged_decode_kernel<64><<<grid, kDecodeWarps * 32, 0, stream>>>(a, e4m3);
+    static_assert(kDecodeCounterBytes >= kDecodeMaxCtas * sizeof(unsigned int), "a counter per CTA");
+    a.row_tiles = (a.group + kRowsMax - 1) / kRowsMax;
+    a.items_per_seq = a.c.heads_kv * a.row_tiles;
+    // no more CTAs than the page table's room could give work to
+    const int64_t room = static_cast<int64_t>(a.c.max_pages) * a.c.page_size;
+    int64_t keys = room;
+    if (a.window > 0 && static_cast<int64_t>(a.window) + a.sinks < room) keys = static_cast<int64_t>(a.window) + a.sinks;
+    const int64_t slices = (keys + kSlice - 1) / kSlice * a.items_per_seq * a.batch;
+    const int64_t worth = (slices + kMinSlices - 1) / kMinSlices;
+    const int64_t most = std::min<int64_t>(kDecodeMaxCtas, 2 * static_cast<int64_t>(a.sm_count));
+    const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min(most, worth)));
+    cudaError_t e;
+    if (kv_dtype == ODF_DTYPE_E4M3)
+        e = head_dim == 64 ? launch_decode<64, true>(a, grid, stream) : launch_decode<128, true>(a, grid, stream);
     else
-        paged_decode_kernel<128><<<grid, kDecodeWarps * 32, 0, stream>>>(a, e4m3);
-    const cudaError_t e = cudaGetLastError();
+        e = head_dim == 64 ? launch_decode<64, false>(a, grid, stream) : launch_decode<128, false>(a, grid, stream);
     if (e != cudaSuccess) *err = cudaGetErrorString(e);
     return e == cudaSuccess ? ODF_OK : ODF_ERR_CUDA;
 }
