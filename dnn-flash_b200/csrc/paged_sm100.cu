@@ -87,6 +87,8 @@ constexpr int kDecodeMaxCtas = 2 * 148;  // two per SM
 constexpr int kSlice = 16;               // keys
 constexpr int kRowsMax = 16;             // query heads of an item
 constexpr int kMinSlices = 16;           // fewest slices worth a CTA of their own
+constexpr int kAhead = 2;                // slices whose page ids are asked for before their load
+constexpr int kFewItems = 4;             // up to a quarter of the CTAs: a CTA per piece
 constexpr int kMergeCols = 32;           // columns of O joined at a time
 constexpr int kMergeStride = kMergeCols + 8;  // floats: 8 banks from row to row
 
@@ -221,100 +223,139 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
 
     // ---- the run of this CTA
     RunCursor cur;
-    int64_t total, first;
-    int ctas;
+    int64_t total = 0, first = 0;  // slices of all items; this CTA's first one
+    int ctas = 0;
+    int few_piece = -1, few_pieces = 0;  // few items: which piece of its item this CTA has, of how many
     {
         int64_t* plan = reinterpret_cast<int64_t*>(smem + Cfg::kOffPlan);
-        int64_t* wsum = plan + 8;
+        int64_t* wsum = plan + 4;
         const int per = (a.batch + kDecodeThreads - 1) / kDecodeThreads;
         const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
-        int64_t mine = 0;
-        for (int b = b0; b < b1; ++b) {
-            const Visible v = visible_keys(a, __ldg(a.lens + b));
-            mine += max(1, (v.count + kSlice - 1) / kSlice);
-        }
-        mine *= a.items_per_seq;
-        int64_t incl = mine;
+        // Sum of `mine` over all threads, and over those before this one.
+        auto scan = [&](int64_t mine, int64_t* before) {
+            int64_t incl = mine;
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int64_t o = __shfl_up_sync(0xffffffffu, incl, off);
-            if (lane >= off) incl += o;
-        }
-        if (lane == 31) wsum[warp] = incl;
-        __syncthreads();
-        total = 0;
-        int64_t before = incl - mine;
-#pragma unroll
-        for (int w = 0; w < kDecodeWarps; ++w) {
-            if (w < warp) before += wsum[w];
-            total += wsum[w];
-        }
-        const int64_t worth = (total + kMinSlices - 1) / kMinSlices;
-        ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), worth));
-        if (static_cast<int>(blockIdx.x) >= ctas) return;
-        first = run_start(blockIdx.x, total, ctas);
-        if (mine > 0 && first >= before && first < before + mine) {
-            int64_t at = before;
-            for (int b = b0;; ++b) {
-                const Visible v = visible_keys(a, __ldg(a.lens + b));
-                const int n = max(1, (v.count + kSlice - 1) / kSlice);
-                const int64_t all = static_cast<int64_t>(n) * a.items_per_seq;
-                if (first < at + all) {
-                    plan[0] = b;
-                    plan[1] = (first - at) / n;
-                    plan[2] = (first - at) % n;
-                    break;
-                }
-                at += all;
+            for (int off = 1; off < 32; off <<= 1) {
+                const int64_t o = __shfl_up_sync(0xffffffffu, incl, off);
+                if (lane >= off) incl += o;
             }
+            if (lane == 31) wsum[warp] = incl;
+            __syncthreads();
+            int64_t all = 0;
+            *before = incl - mine;
+#pragma unroll
+            for (int w = 0; w < kDecodeWarps; ++w) {
+                if (w < warp) *before += wsum[w];
+                all += wsum[w];
+            }
+            __syncthreads();
+            return all;
+        };
+        auto slices_of = [&](int b) {
+            const Visible v = visible_keys(a, __ldg(a.lens + b));
+            return max(1, (v.count + kSlice - 1) / kSlice);
+        };
+        int64_t mine = 0, before;
+        for (int b = b0; b < b1; ++b) mine += slices_of(b);
+        mine *= a.items_per_seq;
+        total = scan(mine, &before);
+        const int64_t items = static_cast<int64_t>(a.batch) * a.items_per_seq;
+        if (items * kFewItems <= gridDim.x) {
+            // few items: every piece has a CTA of its own, an item's pieces even
+            const int64_t room = gridDim.x - items;
+            const int64_t len = max(static_cast<int64_t>(kMinSlices), (total + room - 1) / room);
+            mine = 0;
+            for (int b = b0; b < b1; ++b) mine += (slices_of(b) + len - 1) / len * a.items_per_seq;
+            ctas = static_cast<int>(scan(mine, &before));
+            if (static_cast<int>(blockIdx.x) >= ctas) return;
+            if (static_cast<int>(blockIdx.x) >= before && static_cast<int>(blockIdx.x) < before + mine) {
+                for (int b = b0;; ++b) {
+                    const int pieces = static_cast<int>((slices_of(b) + len - 1) / len);
+                    const int64_t all = static_cast<int64_t>(pieces) * a.items_per_seq;
+                    if (blockIdx.x < before + all) {
+                        const int at = static_cast<int>(blockIdx.x - before);
+                        plan[0] = b;
+                        plan[1] = at / pieces;
+                        plan[2] = at % pieces;
+                        plan[3] = pieces;
+                        break;
+                    }
+                    before += all;
+                }
+            }
+            __syncthreads();
+            cur.b = static_cast<int>(plan[0]);
+            cur.r = static_cast<int>(plan[1]);
+            few_piece = static_cast<int>(plan[2]);
+            few_pieces = static_cast<int>(plan[3]);
+            cur.enter(a);
+            const int even = (cur.n + few_pieces - 1) / few_pieces;
+            cur.s0 = min(cur.n, few_piece * even);
+            cur.s1 = min(cur.n, cur.s0 + even);
+            cur.left = 0;
+        } else {
+            const int64_t worth = (total + kMinSlices - 1) / kMinSlices;
+            ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), worth));
+            if (static_cast<int>(blockIdx.x) >= ctas) return;
+            first = run_start(blockIdx.x, total, ctas);
+            if (first >= before && first < before + mine) {
+                for (int b = b0;; ++b) {
+                    const int n = slices_of(b);
+                    const int64_t all = static_cast<int64_t>(n) * a.items_per_seq;
+                    if (first < before + all) {
+                        plan[0] = b;
+                        plan[1] = (first - before) / n;
+                        plan[2] = (first - before) % n;
+                        break;
+                    }
+                    before += all;
+                }
+            }
+            __syncthreads();
+            cur.b = static_cast<int>(plan[0]);
+            cur.r = static_cast<int>(plan[1]);
+            cur.s0 = static_cast<int>(plan[2]);
+            cur.left = run_start(blockIdx.x + 1, total, ctas) - first;
+            cur.enter(a);
+            cur.cut();
         }
-        __syncthreads();
-        cur.b = static_cast<int>(plan[0]);
-        cur.r = static_cast<int>(plan[1]);
-        cur.s0 = static_cast<int>(plan[2]);
-        cur.left = run_start(blockIdx.x + 1, total, ctas) - first;
-        cur.enter(a);
-        cur.cut();
     }
 
     // ---- loads: this warp's slices s0 + warp, s0 + warp + 4, ... of every piece, in order
     const uint32_t ring = ptx::smem_u32(smem) + warp * (kStages * Cfg::kStageBytes);
     RunCursor ld = cur;
     int ld_s = ld.s0 + warp;
-    bool ld_more = true;
     int ld_slot = 0;  // ring slot of the next load
-    int ld_page = 0, ld_in_page = 0;
-    bool ld_key = false;
-    // finds the next slice and asks for its page ids: lanes 0-15 stand for its keys' K rows, 16-31
-    // for their V rows
-    auto seek = [&]() {
+    // The slices after the next load, whose page ids are on their way: lanes 0-15 stand for the keys' K
+    // rows, 16-31 for their V rows.  slot_in_page -1: key not seen; head -1: no slice left.
+    int page[kAhead], slot_in_page[kAhead], head[kAhead];
+    auto seek = [&](int i) {
+        head[i] = -1;
         while (ld_s >= ld.s1) {
-            if (!ld.next(a)) {
-                ld_more = false;
-                return;
-            }
+            if (!ld.next(a)) return;
             ld_s = ld.s0 + warp;
         }
+        head[i] = ld.r / a.row_tiles;
         const int u = ld_s * kSlice + (lane & 15);
-        ld_key = u < ld.vis.count;
-        if (ld_key) {
+        slot_in_page[i] = -1;
+        if (u < ld.vis.count) {
             const int j = ld.vis.key(u);
             const int at = static_cast<int>(fast_div(static_cast<uint32_t>(j), a.c.fd_page));
-            ld_in_page = j - at * a.c.page_size;
-            ld_page = __ldg(a.c.table + ld.b * a.c.table_stride + at);
+            slot_in_page[i] = j - at * a.c.page_size;
+            page[i] = __ldg(a.c.table + ld.b * a.c.table_stride + at);
         }
+        ld_s += kDecodeWarps;
     };
     auto load = [&]() {
-        if (ld_more) {
-            const int hk = ld.r / a.row_tiles;
+        if (head[0] >= 0) {
             int64_t off = -1;
-            if (ld_key) {
-                if (ld_page < 0 || ld_page >= a.c.num_pages)
+            if (slot_in_page[0] >= 0) {
+                if (page[0] < 0 || page[0] >= a.c.num_pages)
                     bad_page(a.c);
                 else if (lane < 16)
-                    off = ld_page * a.c.k_page + hk * a.c.k_head + ld_in_page * a.c.k_slot;
+                    off = page[0] * a.c.k_page + head[0] * a.c.k_head + slot_in_page[0] * a.c.k_slot;
                 else
-                    off = ld_page * a.c.v_page + hk * a.c.v_head + ld_in_page * a.c.v_slot;
+                    off = page[0] * a.c.v_page + head[0] * a.c.v_head + slot_in_page[0] * a.c.v_slot;
             }
             const uint32_t seen = __ballot_sync(0xffffffffu, off >= 0);
             if (lane == 0) masks[ld_slot] = seen & 0xffffu;
@@ -332,12 +373,18 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
                 cp_async16(at + Cfg::kTileBytes, a.c.v + (vo < 0 ? 0 : vo + c * 16), vo < 0 ? 0 : 16);
             }
             ld_slot = ld_slot + 1 == kStages ? 0 : ld_slot + 1;
-            ld_s += kDecodeWarps;
-            seek();
+#pragma unroll
+            for (int i = 0; i + 1 < kAhead; ++i) {
+                page[i] = page[i + 1];
+                slot_in_page[i] = slot_in_page[i + 1];
+                head[i] = head[i + 1];
+            }
+            seek(kAhead - 1);
         }
         cp_async_commit();  // an empty group when there is nothing left, so that the count below holds
     };
-    seek();
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) seek(i);
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) load();
 
@@ -597,36 +644,49 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
                 a.lse[static_cast<int64_t>(cur.b) * a.heads_q + h0 + r] =
                     sum == 0.0f ? -INFINITY : (mr + (log2f(sum) - kShift)) * kLn2;
         };
-#pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += kMergeCols) {
+        // A strip is four column blocks: bf16 columns 8 j + n, in order; 8-bit features (D/8) n + j, four
+        // in a row for each n.  With at most 8 rows the other half of the buffer takes every second strip.
+        const int other = rows <= 8 ? 8 * kMergeStride : 0;
 #pragma unroll
-            for (int j = 0; j < kBlocks; ++j) {
+        for (int q4 = 0; q4 < kBlocks / 4; ++q4) {
+            float* buf = merge + ((q4 & 1) ? other : 0);
+            if (q4 > 0 && other == 0) __syncthreads();  // the strip before has been read
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = g + 8 * (i >> 1);
-                    const int d = kE4M3 ? (D / 8) * (2 * t + (i & 1)) + j : 8 * j + 2 * t + (i & 1);
-                    if (r < rows && d >= c0 && d < c0 + kMergeCols)
-                        merge[(warp * kRowsMax + r) * kMergeStride + d - c0] = o[j][i];
+            for (int hf = 0; hf < 2; ++hf) {
+                const int r = g + 8 * hf;
+                float* dst = buf + (warp * kRowsMax + r) * kMergeStride;
+                if (r < rows) {
+                    if constexpr (kE4M3) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            *reinterpret_cast<float4*>(dst + (2 * t + i) * 4) =
+                                make_float4(o[4 * q4][2 * hf + i], o[4 * q4 + 1][2 * hf + i], o[4 * q4 + 2][2 * hf + i],
+                                            o[4 * q4 + 3][2 * hf + i]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            *reinterpret_cast<float2*>(dst + 8 * j + 2 * t) = make_float2(o[4 * q4 + j][2 * hf], o[4 * q4 + j][2 * hf + 1]);
+                    }
                 }
             }
             __syncthreads();
             if (row_ok) {
-                const int col = (threadIdx.x & 7) * 4;
+                const int c4 = threadIdx.x & 7;
                 float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int w = 0; w < kDecodeWarps; ++w) {
-                    const float4 y = *reinterpret_cast<const float4*>(merge + (w * kRowsMax + row) * kMergeStride + col);
+                    const float4 y = *reinterpret_cast<const float4*>(buf + (w * kRowsMax + row) * kMergeStride + 4 * c4);
                     x.x += wt[w] * y.x;
                     x.y += wt[w] * y.y;
                     x.z += wt[w] * y.z;
                     x.w += wt[w] * y.w;
                 }
+                const int d = kE4M3 ? (D / 8) * c4 + 4 * q4 : kMergeCols * q4 + 4 * c4;
                 if (whole)
-                    write_out(row, c0 + col, x, L);
+                    write_out(row, d, x, L);
                 else
-                    *reinterpret_cast<float4*>(part + row * D + c0 + col) = x;
+                    *reinterpret_cast<float4*>(part + row * D + d) = x;
             }
-            __syncthreads();
         }
         if (row_ok && (threadIdx.x & 7) == 0) {
             if (whole) {
@@ -637,45 +697,111 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
             }
         }
         if (!whole) {
-            const int c_first = run_owner(item0, total, ctas);
-            const int pieces = run_owner(item0 + cur.n - 1, total, ctas) - c_first + 1;
-            __threadfence();
-            __syncthreads();
-            int* last = reinterpret_cast<int*>(stat_m);
+            const int c_first = few_piece >= 0 ? static_cast<int>(blockIdx.x) - few_piece : run_owner(item0, total, ctas);
+            const int pieces = few_piece >= 0 ? few_pieces : run_owner(item0 + cur.n - 1, total, ctas) - c_first + 1;
+            __syncthreads();  // the CTA's part is written, as seen from its first thread
+            int* last = reinterpret_cast<int*>(smem + Cfg::kOffPlan);
             if (threadIdx.x == 0) {
+                __threadfence();
                 const unsigned int old =
                     atomicInc(static_cast<unsigned int*>(a.workspace) + c_first, static_cast<unsigned int>(pieces - 1));
+                __threadfence();
                 *last = old == static_cast<unsigned int>(pieces - 1);
             }
             __syncthreads();
             const bool join = *last != 0;
             __syncthreads();
-            if (join && row_ok) {
-                __threadfence();
-                const float* p0 = slots + (2 * static_cast<int64_t>(c_first) + 1) * kSlotFloats;  // the first piece
-                auto piece = [&](int k) { return k == 0 ? p0 : slots + 2 * static_cast<int64_t>(c_first + k) * kSlotFloats; };
+            if (join) {
+                auto piece = [&](int k) {
+                    return slots + (2 * static_cast<int64_t>(c_first + k) + (k == 0 ? 1 : 0)) * kSlotFloats;
+                };
+                // the pieces' weights by row (8 threads to a row), then O, float4 units of the rows spread
+                // over the threads (with few rows, the pieces too) so that many loads are in flight
+                constexpr int kHeld = kDecodeWarps * kMergeStride;
+                float* wts = merge;  // [min(pieces, kHeld)][kRowsMax]
                 float mj = -INFINITY, lj = 0.0f;
-                for (int k = 0; k < pieces; ++k) mj = fmaxf(mj, __ldcg(piece(k) + kRowsMax * D + row));
-                float4 x[D / 32];
+#pragma unroll 4
+                for (int k = threadIdx.x & 7; k < pieces; k += 8) {
+                    const float mk = __ldcg(piece(k) + kRowsMax * D + row);
+                    const float lk = __ldcg(piece(k) + kRowsMax * D + kRowsMax + row);
+                    if (k < kHeld) wts[k * kRowsMax + row] = mk;
+                    const float mn = fmaxf(mj, mk);
+                    if (mn != -INFINITY) lj = lj * ptx::ex2(mj - mn) + lk * ptx::ex2(mk - mn);
+                    else lj += lk;  // 0, or NaN
+                    mj = mn;
+                }
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int k = 0; k < pieces; ++k) {
-                    const float* pk = piece(k);
-                    const float mk = __ldcg(pk + kRowsMax * D + row);
-                    const float w = mk == -INFINITY ? 0.0f : ptx::ex2(mk - mj);
-                    lj += w * __ldcg(pk + kRowsMax * D + kRowsMax + row);
+                for (int off = 4; off > 0; off >>= 1) {
+                    const float mo = __shfl_xor_sync(0xffffffffu, mj, off), lo = __shfl_xor_sync(0xffffffffu, lj, off);
+                    const float mn = fmaxf(mj, mo);
+                    lj = mn == -INFINITY ? lj + lo : lj * ptx::ex2(mj - mn) + lo * ptx::ex2(mo - mn);
+                    mj = mn;
+                }
+                for (int k = threadIdx.x & 7; k < min(pieces, kHeld); k += 8) {
+                    const float mk = wts[k * kRowsMax + row];
+                    wts[k * kRowsMax + row] = mk == -INFINITY ? 0.0f : ptx::ex2(mk - mj);
+                }
+                if ((threadIdx.x & 7) == 0) {
+                    stat_m[row] = mj;
+                    stat_l[row] = lj;
+                }
+                if (row_ok && (threadIdx.x & 7) == 0) write_lse(row, mj, lj);
+                __syncthreads();
+                constexpr int kUnitsMax = kRowsMax * (D / 4) / kDecodeThreads;  // per thread
+                const int units = rows * (D / 4);
+                const int groups = units >= kDecodeThreads ? 1 : kDecodeThreads / units;
+                const int grp = static_cast<int>(threadIdx.x) / units;
+                const int u0 = groups > 1 ? static_cast<int>(threadIdx.x) - grp * units : static_cast<int>(threadIdx.x);
+                float4 x[kUnitsMax];
 #pragma unroll
-                    for (int i = 0; i < D / 32; ++i) {
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(pk + row * D + i * 32) + (threadIdx.x & 7));
-                        x[i].x += w * y.x;
-                        x[i].y += w * y.y;
-                        x[i].z += w * y.z;
-                        x[i].w += w * y.w;
+                for (int i = 0; i < kUnitsMax; ++i) x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (grp < groups || groups == 1) {
+#pragma unroll 8
+                    for (int k = groups > 1 ? grp : 0; k < pieces; k += groups) {
+                        const float4* pk = reinterpret_cast<const float4*>(piece(k));
+#pragma unroll
+                        for (int i = 0; i < kUnitsMax; ++i) {
+                            const int u = u0 + i * kDecodeThreads;
+                            if (u < units) {
+                                const float4 y = __ldcg(pk + u);
+                                const int r = u / (D / 4);
+                                float w;
+                                if (k < kHeld) {
+                                    w = wts[k * kRowsMax + r];
+                                } else {  // one item over most of the GPU
+                                    const float mk = __ldcg(piece(k) + kRowsMax * D + r);
+                                    w = mk == -INFINITY ? 0.0f : ptx::ex2(mk - stat_m[r]);
+                                }
+                                x[i].x += w * y.x;
+                                x[i].y += w * y.y;
+                                x[i].z += w * y.z;
+                                x[i].w += w * y.w;
+                            }
+                        }
+                    }
+                }
+                if (groups > 1) {
+                    __syncthreads();  // the weights have been read
+                    float4* sums = reinterpret_cast<float4*>(merge);
+                    if (grp < groups) sums[grp * units + u0] = x[0];
+                    __syncthreads();
+                    if (grp == 0) {
+                        for (int k = 1; k < groups; ++k) {
+                            const float4 y = sums[k * units + u0];
+                            x[0].x += y.x;
+                            x[0].y += y.y;
+                            x[0].z += y.z;
+                            x[0].w += y.w;
+                        }
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) write_out(row, i * 32 + (threadIdx.x & 7) * 4, x[i], lj);
-                if ((threadIdx.x & 7) == 0) write_lse(row, mj, lj);
+                for (int i = 0; i < kUnitsMax; ++i) {
+                    const int u = u0 + i * kDecodeThreads;
+                    if (u < units && (groups == 1 || grp == 0))
+                        write_out(u / (D / 4), (u % (D / 4)) * 4, x[i], stat_l[u / (D / 4)]);
+                }
+                __syncthreads();
             }
         }
         item0 += cur.n;
@@ -805,7 +931,9 @@ int launch_paged_decode(DecodeArgs& a, int32_t head_dim, int32_t kv_dtype, cudaS
     int64_t keys = room;
     if (a.window > 0 && static_cast<int64_t>(a.window) + a.sinks < room) keys = static_cast<int64_t>(a.window) + a.sinks;
     const int64_t slices = (keys + kSlice - 1) / kSlice * a.items_per_seq * a.batch;
-    const int64_t worth = (slices + kMinSlices - 1) / kMinSlices;
+    // and as many as give every piece of few items one of its own
+    const int64_t worth =
+        std::max((slices + kMinSlices - 1) / kMinSlices, static_cast<int64_t>(kFewItems) * a.items_per_seq * a.batch);
     const int64_t most = std::min<int64_t>(kDecodeMaxCtas, 2 * static_cast<int64_t>(a.sm_count));
     const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min(most, worth)));
     cudaError_t e;

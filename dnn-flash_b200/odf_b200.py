@@ -35,6 +35,7 @@ ODF_BIAS_SAME_SHAPE = 1
 ODF_BIAS_ALIBI = 4
 TILE_Q = 128
 TILE_K = 128
+_INT64_MAX = 2 ** 63 - 1
 
 
 class FwdParams(C.Structure):
@@ -303,38 +304,27 @@ def flash_fwd_window(q, k, v, *, window, sinks=0, q_offset=0, scale=None, alibi=
         raise ValueError("q must be [B, Hq, M, D], k and v of one shape [B, Hkv, N, D]")
     if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
         raise ValueError("q, k and v must be bfloat16")
+    B, Hq, M, D = q.shape
     dev = q.device
     _require_cuda(dev)
     _on(k, "k", dev)
     _on(v, "v", dev)
-    B, Hq, M, D = q.shape
-    if alibi_slopes is not None and len(alibi_slopes) != Hq:
-        raise ValueError("alibi_slopes needs one slope per query head")
-    with _launch_on(dev, stream) as handle:
-        if out is None:
-            out = torch.empty((B, Hq, M, D), dtype=out_dtype or torch.float32, device=dev)
-        lse = lse_out
-        if want_lse and lse is None:
-            lse = torch.empty((B, Hq, M), dtype=torch.float32, device=dev)
-        _on(out, "out", dev)
-        _on(lse, "lse_out", dev)
-        if out.shape != q.shape or out.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError("out must be float32 or bfloat16 of q's shape")
-        if lse is not None and (lse.shape != (B, Hq, M) or lse.dtype != torch.float32 or not lse.is_contiguous()):
-            raise ValueError("lse_out must be contiguous float32 [B, Hq, M]")
-        p, keep = fill_params(q, k, v, out, lse, causal=True, scale=1.0 / math.sqrt(D) if scale is None else scale,
-                              block_mask=None, mask_block=None, alibi=alibi, alibi_slopes_host=alibi_slopes,
-                              softcap=softcap, workspace=None, visits=None)
-        for field, t, name in ((p.q_strides, q, "q"), (p.k_strides, k, "k"), (p.v_strides, v, "v"), (p.o_strides, out, "out")):
-            for i, s in enumerate(_dense_strides(t, name)):
-                field[i] = s
-        w = Window(window, sinks, q_offset)
+    slopes = _slopes_array(alibi_slopes, Hq) if alibi else None
+    where, handle = _launch_on(dev, stream)
+    with where:
+        out, lse = _outputs(q, out, lse_out, out_dtype, want_lse, dev)
+        p = FwdParams(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+                      ODF_DTYPE_BF16, ODF_DTYPE_BF16 if out.dtype == torch.bfloat16 else ODF_DTYPE_F32, B, Hq, k.shape[1], M,
+                      k.shape[2], D, D, _strides(q, "q"), _strides(k, "k"), _strides(v, "v"), _strides(out, "out"),
+                      1.0 / math.sqrt(D) if scale is None else scale, 1, None, 0, 0, 0, 0,
+                      ODF_BIAS_ALIBI if alibi else ODF_BIAS_NONE, None if slopes is None else C.addressof(slopes), softcap)
+        w = Window(min(window, _INT64_MAX), min(sinks, _INT64_MAX), q_offset)
         nbytes = lib.odf_fwd_window_workspace_size(C.byref(p), C.byref(w))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 256 else None
-        if ws is not None:
+        ws = None
+        if nbytes > 256:  # room for the parts of a split key range
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
         _check(lib.odf_flash_fwd_window_sm100(C.byref(p), C.byref(w), handle))
-    del keep
     return out, (lse if want_lse else None)
 
 
@@ -408,100 +398,160 @@ def tile_map(seqlen_q, seqlen_k, causal, block_mask=None, mask_block=(128, 128),
 
 
 # ------------------------------------------------------------------ paged key-value cache
+# A decode step makes these calls once per layer, so they are written for few Python steps: structs are
+# filled in one constructor call, contiguous tensors pass zero strides, and the device and stream are
+# only switched where they differ from the current ones.
+_NO_STRIDES3 = (C.c_int64 * 3)()
+_NO_STRIDES2 = (C.c_int64 * 2)()
+
+
+def _strides(t, name):
+    """Element strides of all dimensions but the last, which must be contiguous; all zero = contiguous."""
+    n = t.dim() - 1
+    if t.is_contiguous():
+        return _NO_STRIDES3 if n == 3 else _NO_STRIDES2
+    shape, stride = t.shape, t.stride()
+    if stride[n] != 1:
+        raise ValueError(f"the innermost (feature) dimension of {name} must be contiguous")
+    out, dense = list(stride[:n]), shape[n]
+    for i in range(n - 1, -1, -1):  # a dimension of size 1 has no stride of its own: a contiguous tensor's
+        if shape[i] == 1:
+            out[i] = dense
+        dense *= shape[i]
+    return (C.c_int64 * n)(*out)
+
+
 def _on(tensor, name, device):
-    if tensor is not None and tensor.device != device:
+    if tensor.device != device:
         raise ValueError(f"{name} is on {tensor.device}, the call runs on {device}")
 
 
-def _int32_on(tensor, name, device, shape):
-    """A contiguous int32 device tensor of the given shape (None where a size is free)."""
+def _int32(tensor, name, device, rows):
+    """Address of a contiguous int32 device vector of `rows` elements."""
     import torch
 
+    if tensor.dtype != torch.int32 or tensor.shape != (rows,) or not tensor.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape [{rows}], got {tensor.dtype} {list(tensor.shape)}")
     _on(tensor, name, device)
-    if tensor.dtype != torch.int32 or tensor.dim() != len(shape) or any(
-            n is not None and n != m for n, m in zip(shape, tensor.shape)):
-        raise ValueError(f"{name} must be int32 of shape {list(shape)}, got {tensor.dtype} {list(tensor.shape)}")
-    if tensor.stride(-1) != 1 and tensor.shape[-1] > 1:
-        raise ValueError(f"{name} must be contiguous in its last dimension")
     return tensor.data_ptr()
 
 
-def _dense_strides(t, name):
-    """Strides of all dimensions but the last, which must be contiguous.  A dimension of size 1 has
-    no stride of its own; it gets the one a contiguous tensor would have."""
-    if t.stride(-1) != 1:
-        raise ValueError(f"the innermost (feature) dimension of {name} must be contiguous")
-    out, dense = [], 1
-    for n, s in zip(reversed(t.shape), reversed(t.stride())):
-        out.append(dense if n == 1 else s)
-        dense *= n
-    return list(reversed(out))[:-1]
-
-
-def _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, batch):
+def _scale_ptr(tensor, name, device, heads):
     import torch
 
-    if k_pages.dim() != 4 or v_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+    if tensor is None:
+        return None
+    if tensor.dtype != torch.float32 or tensor.shape != (heads,) or not tensor.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 tensor [{heads}]")
+    _on(tensor, name, device)
+    return tensor.data_ptr()
+
+
+def _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, device, batch, heads=None, head_dim=None):
+    """odf_paged_cache of one layer's pages (PagedCache), checked against the call's other tensors."""
+    import torch
+
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError("k_pages and v_pages must be rank 4 [pages, heads_kv, page_size, head_dim] of one shape")
-    if k_pages.dtype != v_pages.dtype:
-        raise ValueError("k_pages and v_pages must have one dtype")
-    c = PagedCache()
-    c.k_pages, c.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
-    if k_pages.dtype == torch.bfloat16:
-        c.kv_dtype = ODF_DTYPE_BF16
-    elif k_pages.dtype == torch.float8_e4m3fn:
-        c.kv_dtype = ODF_DTYPE_E4M3
-    else:
-        raise ValueError(f"a cache holds bfloat16 or float8_e4m3fn, not {k_pages.dtype}")
-    dev = k_pages.device
-    _on(v_pages, "v_pages", dev)
-    c.num_pages, c.heads_kv, c.page_size, c.head_dim = k_pages.shape
-    for field, t, name in ((c.k_strides, k_pages, "k_pages"), (c.v_strides, v_pages, "v_pages")):
-        for i, s in enumerate(_dense_strides(t, name)):
-            field[i] = s
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t is not None:
-            _on(t, name, dev)
-            if t.dtype != torch.float32 or t.shape != (c.heads_kv,) or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous float32 tensor [heads_kv]")
-            setattr(c, name, t.data_ptr())
+    if v_pages.dtype != dtype or dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+        raise ValueError(f"a cache holds bfloat16 or float8_e4m3fn, not {dtype} and {v_pages.dtype}")
+    _on(k_pages, "k_pages", device)
+    _on(v_pages, "v_pages", device)
+    pages, hkv, page_size, dim = shape
+    if (heads is not None and heads != hkv) or (head_dim is not None and head_dim != dim):
+        raise ValueError("the new tensors and the cache must have the same kv-heads and head_dim")
+    table, table_stride, max_pages = None, 0, 0
     if page_table is not None:
-        c.page_table = _int32_on(page_table, "page_table", dev, (batch, None))
-        c.max_pages = page_table.shape[1]
-        c.table_stride = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
-    return c
+        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
+            raise ValueError(f"page_table must be int32 [{batch}, max_pages], got {page_table.dtype} {list(page_table.shape)}")
+        max_pages = page_table.shape[1]
+        if not page_table.is_contiguous():
+            if page_table.stride(1) != 1 and max_pages > 1:
+                raise ValueError("page_table must be contiguous in its last dimension")
+            table_stride = page_table.stride(0) if batch > 1 else 0
+            if batch > 1 and table_stride < max_pages:  # rows that overlap, an expanded table among them
+                raise ValueError("page_table rows must not overlap")
+        _on(page_table, "page_table", device)
+        table = page_table.data_ptr()
+    return PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), ODF_DTYPE_BF16 if dtype == torch.bfloat16 else ODF_DTYPE_E4M3,
+                      pages, hkv, page_size, dim, _strides(k_pages, "k_pages"), _strides(v_pages, "v_pages"),
+                      _scale_ptr(k_scale, "k_scale", device, hkv), _scale_ptr(v_scale, "v_scale", device, hkv),
+                      table, table_stride, max_pages)
 
 
-class _launch_on:
-    """Makes `device` current and yields the stream handle to launch on; temporaries and outputs
-    allocated inside belong to that stream."""
+class _StayHere:
+    def __enter__(self):
+        return self
 
-    def __init__(self, device, stream):
+    def __exit__(self, *exc):
+        return False
+
+
+_STAY_HERE = _StayHere()
+
+
+class _SwitchTo:
+    """Makes a device and a stream current, so that what is allocated inside belongs to that stream."""
+
+    def __init__(self, device, handle):
         import torch
 
         self.device = torch.cuda.device(device)
-        current = torch.cuda.current_stream(device)
-        self.handle = current.cuda_stream if stream is None else getattr(stream, "cuda_stream", stream)
-        self.stream = None
-        if self.handle != current.cuda_stream:
-            self.stream = torch.cuda.stream(torch.cuda.ExternalStream(self.handle, device=device) if self.handle
-                                            else torch.cuda.default_stream(device))
+        self.stream = torch.cuda.stream(torch.cuda.ExternalStream(handle, device=device) if handle
+                                        else torch.cuda.default_stream(device))
 
     def __enter__(self):
         self.device.__enter__()
-        if self.stream is not None:
-            self.stream.__enter__()
-        return C.c_void_p(self.handle)
+        self.stream.__enter__()
 
     def __exit__(self, *exc):
-        if self.stream is not None:
-            self.stream.__exit__(*exc)
+        self.stream.__exit__(*exc)
         return self.device.__exit__(*exc)
+
+
+def _launch_on(device, stream):
+    """(context, stream handle) for a launch on `device` and `stream` (a handle, a torch stream or None
+    for torch's current one)."""
+    import torch
+
+    # the raw forms of torch.cuda.current_stream(device).cuda_stream and current_device(), which cost 4 us more
+    current = torch._C._cuda_getCurrentRawStream(device.index)
+    handle = current if stream is None else getattr(stream, "cuda_stream", stream)
+    if handle == current and torch._C._cuda_getDevice() == device.index:
+        return _STAY_HERE, handle
+    return _SwitchTo(device, handle), handle
 
 
 def _require_cuda(device):
     if device.type != "cuda":
         raise ValueError(f"tensors must be on a CUDA device, not {device}")
+
+
+def _outputs(q, out, lse_out, out_dtype, want_lse, device):
+    """The given or new outputs of an attention call with q's shape."""
+    import torch
+
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype or torch.float32, device=device)
+    else:
+        _on(out, "out", device)
+    if out.shape != q.shape or out.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("out must be float32 or bfloat16 of q's shape")
+    if lse_out is None:
+        return out, torch.empty(q.shape[:-1], dtype=torch.float32, device=device) if want_lse else None
+    _on(lse_out, "lse_out", device)
+    if lse_out.shape != q.shape[:-1] or lse_out.dtype != torch.float32 or not lse_out.is_contiguous():
+        raise ValueError("lse_out must be contiguous float32 of q's shape without its last dimension")
+    return out, lse_out
+
+
+def _slopes_array(alibi_slopes, heads):
+    if alibi_slopes is None:
+        return None
+    if len(alibi_slopes) != heads:
+        raise ValueError("alibi_slopes needs one slope per query head")
+    return (C.c_float * heads)(*[float(x) for x in alibi_slopes])
 
 
 def paged_decode_workspace(batch, heads_q, heads_kv, head_dim, device="cuda"):
@@ -529,52 +579,27 @@ def paged_decode(q, k_pages, v_pages, page_table, lens, *, scale=None, window=0,
     """
     import torch
 
-    lib = load_library()
     if q.dim() != 3 or q.dtype != torch.bfloat16:
         raise ValueError("q must be bfloat16 of rank 3 [B, Hq, D]")
     B, Hq, D = q.shape
     dev = q.device
     _require_cuda(dev)
-    _on(k_pages, "k_pages", dev)
-    if k_pages.dim() == 4 and k_pages.shape[3] != D:
-        raise ValueError("q and the cache must have one head_dim")
-    p = DecodeParams()
-    p.cache = _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, B)
-    p.q, p.lens = q.data_ptr(), _int32_on(lens, "lens", dev, (B,))
-    p.batch, p.heads_q = B, Hq
-    p.scale = 1.0 / math.sqrt(D) if scale is None else scale
-    p.window, p.sinks, p.softcap = window, sinks, softcap
-    keep = None
-    if alibi:
-        p.bias_kind = ODF_BIAS_ALIBI
-        if alibi_slopes is not None:
-            if len(alibi_slopes) != Hq:
-                raise ValueError("alibi_slopes needs one slope per query head")
-            keep = (C.c_float * Hq)(*[float(x) for x in alibi_slopes])
-            p.alibi_slopes = C.cast(keep, C.c_void_p)
-    with _launch_on(dev, stream) as handle:
-        if out is None:
-            out = torch.empty((B, Hq, D), dtype=out_dtype or torch.float32, device=dev)
-        lse = lse_out
-        if want_lse and lse is None:
-            lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
-        _on(out, "out", dev)
-        _on(lse, "lse_out", dev)
-        if out.shape != q.shape or out.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError("out must be float32 or bfloat16 of q's shape")
-        if lse is not None and (lse.shape != (B, Hq) or lse.dtype != torch.float32 or not lse.is_contiguous()):
-            raise ValueError("lse_out must be contiguous float32 [B, Hq]")
-        p.o, p.o_dtype = out.data_ptr(), ODF_DTYPE_BF16 if out.dtype == torch.bfloat16 else ODF_DTYPE_F32
-        p.lse = lse.data_ptr() if lse is not None else None
-        for field, t, name in ((p.q_strides, q, "q"), (p.o_strides, out, "out")):
-            for i, s in enumerate(_dense_strides(t, name)):
-                field[i] = s
+    cache = _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, dev, B, head_dim=D)
+    lens_ptr = _int32(lens, "lens", dev, B)
+    slopes = _slopes_array(alibi_slopes, Hq) if alibi else None
+    where, handle = _launch_on(dev, stream)
+    with where:
+        out, lse = _outputs(q, out, lse_out, out_dtype, want_lse, dev)
         if workspace is None:
-            workspace = paged_decode_workspace(B, Hq, p.cache.heads_kv, D, device=dev)
-        _on(workspace, "workspace", dev)
-        p.workspace, p.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        _check(lib.odf_paged_decode_sm100(C.byref(p), handle))
-    del keep
+            workspace = paged_decode_workspace(B, Hq, cache.heads_kv, D, device=dev)
+        else:
+            _on(workspace, "workspace", dev)
+        p = DecodeParams(q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+                         ODF_DTYPE_BF16 if out.dtype == torch.bfloat16 else ODF_DTYPE_F32, B, Hq, _strides(q, "q"),
+                         _strides(out, "out"), lens_ptr, cache, 1.0 / math.sqrt(D) if scale is None else scale,
+                         min(window, _INT64_MAX), min(sinks, _INT64_MAX), ODF_BIAS_ALIBI if alibi else ODF_BIAS_NONE,
+                         None if slopes is None else C.addressof(slopes), softcap, workspace.data_ptr(), workspace.nbytes)
+        _check(load_library().odf_paged_decode_sm100(C.byref(p), handle))
     return out, (lse if want_lse else None)
 
 
@@ -586,26 +611,18 @@ def paged_append(k, v, k_pages, v_pages, page_table, starts, *, counts=None, k_s
     """
     import torch
 
-    lib = load_library()
     if k.dim() != 4 or k.shape != v.shape or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise ValueError("k and v must be bfloat16 of one rank 4 shape [B, Hkv, T, D]")
     B, Hkv, T, D = k.shape
     dev = k.device
     _require_cuda(dev)
     _on(v, "v", dev)
-    _on(k_pages, "k_pages", dev)
-    if k_pages.dim() == 4 and (k_pages.shape[1] != Hkv or k_pages.shape[3] != D):
-        raise ValueError("k and the cache must have the same kv-heads and head_dim")
-    p = AppendParams()
-    p.cache = _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, B)
-    p.k, p.v, p.batch, p.tokens = k.data_ptr(), v.data_ptr(), B, T
-    for field, t, name in ((p.k_strides, k, "k"), (p.v_strides, v, "v")):
-        for i, s in enumerate(_dense_strides(t, name)):
-            field[i] = s
-    p.starts = _int32_on(starts, "starts", dev, (B,))
-    p.counts = _int32_on(counts, "counts", dev, (B,)) if counts is not None else None
-    with _launch_on(dev, stream) as handle:
-        _check(lib.odf_paged_append_sm100(C.byref(p), handle))
+    cache = _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, dev, B, Hkv, D)
+    p = AppendParams(k.data_ptr(), v.data_ptr(), B, T, _strides(k, "k"), _strides(v, "v"), _int32(starts, "starts", dev, B),
+                     None if counts is None else _int32(counts, "counts", dev, B), cache)
+    where, handle = _launch_on(dev, stream)
+    with where:
+        _check(load_library().odf_paged_append_sm100(C.byref(p), handle))
 
 
 def page_copy(k_pages, v_pages, pairs, *, stream=None):
@@ -617,30 +634,29 @@ def page_copy(k_pages, v_pages, pairs, *, stream=None):
     """
     import numpy as np
 
-    lib = load_library()
-    if k_pages.dim() not in (4, 5) or k_pages.shape != v_pages.shape:
+    layered = k_pages.dim() == 5
+    if k_pages.dim() not in (4, 5) or k_pages.shape != v_pages.shape or (layered and k_pages.shape[0] == 0):
         raise ValueError("k_pages and v_pages must be [pages, Hkv, page_size, D] or [layers, pages, ...] of one shape")
     dev = k_pages.device
     _require_cuda(dev)
     ids = np.asarray(pairs)
     if ids.size == 0:
-        ids = np.zeros((0, 2), dtype=np.int32)
-    if ids.ndim != 2 or ids.shape[1] != 2 or not np.issubdtype(ids.dtype, np.integer):
+        return
+    if ids.ndim != 2 or ids.shape[1] != 2 or ids.dtype.kind not in "iu":
         raise ValueError("pairs must be integers of shape [n, 2]")
-    if ids.size and (ids.min() < 0 or ids.max() >= k_pages.shape[-4]):
-        raise ValueError("a page id is outside the cache")
-    ids = np.ascontiguousarray(ids, dtype=np.int32)
-    p = PageCopyParams()
-    layered = k_pages.dim() == 5
-    if layered and k_pages.shape[0] == 0:
-        raise ValueError("the cache has no layers")
-    p.cache = _cache_params(k_pages[0] if layered else k_pages, v_pages[0] if layered else v_pages, None, None, None, 0)
-    p.layers = k_pages.shape[0] if layered else 1
+    if ids.dtype != np.int32:
+        if int(ids.min()) < 0 or int(ids.max()) >= k_pages.shape[-4]:  # before they are cut to 32 bits
+            raise ValueError("a page id is outside the cache")
+        ids = ids.astype(np.int32)
+    ids = np.ascontiguousarray(ids)
     if layered:
-        p.k_layer_stride, p.v_layer_stride = k_pages.stride(0), v_pages.stride(0)
-    p.pairs, p.n_pairs = ids.ctypes.data, len(ids)
-    with _launch_on(dev, stream) as handle:
-        _check(lib.odf_page_copy_sm100(C.byref(p), handle))
+        cache = _cache_params(k_pages[0], v_pages[0], None, None, None, dev, 0)
+        p = PageCopyParams(cache, k_pages.shape[0], k_pages.stride(0), v_pages.stride(0), ids.ctypes.data, len(ids))
+    else:
+        p = PageCopyParams(_cache_params(k_pages, v_pages, None, None, None, dev, 0), 1, 0, 0, ids.ctypes.data, len(ids))
+    where, handle = _launch_on(dev, stream)
+    with where:
+        _check(load_library().odf_page_copy_sm100(C.byref(p), handle))
 
 
 class PagePool:
