@@ -141,6 +141,14 @@ int odf_paged_decode_sm100(const odf_decode_params* p, void* stream) {
         return set_error(ODF_ERR_INVALID_ARG, "heads_q must be a multiple of heads_kv");
     if (p->batch > 0x7fffff || p->heads_q > 65535 || p->batch * p->heads_q > 0x7fffffffLL)
         return set_error(ODF_ERR_UNSUPPORTED, "batch or heads beyond the kernel's limits");
+    // the kernel counts rows of the cache in 16-byte units of 32 bits
+    for (int which = 0; which < 2; ++which) {
+        const double reach = static_cast<double>(which ? a.c.v_page : a.c.k_page) * (a.c.num_pages - 1) +
+                             static_cast<double>(which ? a.c.v_head : a.c.k_head) * (a.c.heads_kv - 1) +
+                             static_cast<double>(which ? a.c.v_slot : a.c.k_slot) * (a.c.page_size - 1) + 256.0;
+        if (reach > 16.0 * 4294967295.0)
+            return set_error(ODF_ERR_UNSUPPORTED, "K or V pages of one layer span more than 64 GB");
+    }
     if (p->o_dtype != ODF_DTYPE_F32 && p->o_dtype != ODF_DTYPE_BF16)
         return set_error(ODF_ERR_UNSUPPORTED, "output dtype must be f32 or bf16");
     if (!std::isfinite(p->scale)) return set_error(ODF_ERR_INVALID_ARG, "scale must be finite");

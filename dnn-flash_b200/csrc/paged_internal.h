@@ -27,22 +27,24 @@ struct PagedView {
 
 struct DecodeArgs {
     PagedView c;
+    // the cache's strides in 16-byte units
+    uint32_t k16_page, k16_head, k16_slot, v16_page, v16_head, v16_slot;
+    const int32_t* lens;
+    int32_t batch, heads_q, group;
+    int32_t row_tiles, items_per_seq;  // items of one sequence: kv-heads x blocks of query heads
+    FastDiv fd_items;                  // by items_per_seq
+    int32_t window, sinks;             // window 0 = every key
     const void* q;
     int64_t q_b, q_h;  // elements
     void* o;
     int64_t o_b, o_h;  // elements
     float* lse;
-    const int32_t* lens;
-    int32_t o_bf16;
-    int32_t batch, heads_q, group;
+    void* workspace;
+    int32_t o_bf16, sm_count;
     float scale;
     float softcap, inv_softcap;
-    int32_t window, sinks;  // window 0 = every key
     int32_t has_alibi, alibi_generated;
     float alibi_slopes[ODF_MAX_EXPLICIT_SLOPES];
-    void* workspace;
-    int32_t sm_count;
-    int32_t row_tiles, items_per_seq;  // items of one sequence: kv-heads x tiles of 16 query heads
 };
 
 struct AppendArgs {

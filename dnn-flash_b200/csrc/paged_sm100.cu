@@ -66,54 +66,66 @@ __device__ __forceinline__ bool row_offsets(const PagedView& c, const int32_t* t
 //
 // What bounds it is the cache: every visible key and value is read once (2 d e bytes a key and
 // kv-head) against 4 d FLOP per query head, at most a few dozen FLOP a byte, so the kernel is built
-// around keeping loads in flight and the arithmetic behind them is one m16n8k16 product per 16
-// keys (S = Q K^T, then O += P V, the query heads of one kv-head as the 16 rows).  tcgen05 would
-// want 128 rows; there are at most 16, and the warp-level product keeps up (at d = 128 a key costs two
-// of them, against 22 clocks that its 512 bytes take at the SM's share of HBM).
+// around keeping loads in flight and short chains of arithmetic behind them.
 //
-// Work: an item is (sequence, kv-head, 16 query heads); its visible keys are cut into slices of 16.  The slices
-// of all items in a row are dealt to the CTAs in equal consecutive runs, whatever the lengths, by a
-// prefix sum over the lengths that every CTA does for itself.  A run holds pieces of one or
-// several items; an item that lies in one run is written out directly, the pieces of one that
-// does not go to the workspace as fp32 O, max and sum, and the CTA that is last to finish (a
-// counter that wraps to zero) joins them in order, so the result does not depend on who that is.
+// Products are warp-level m16n8k16 with the keys as the 16 rows: S^T = K Q^T, then O^T += V^T P^T, the
+// query heads of one kv-head as the 8 columns (one block of them up to 8 heads, else two).  tcgen05 would
+// want 128 rows of keys by 8 columns through tensor memory; the warp-level product leaves the tensor
+// pipe a quarter busy and needs no hand-over between warps.
+//
+// Work: an item is (sequence, kv-head, block of query heads); its visible keys are cut into slices of 16 or
+// 32.  The slices of all items in a row are dealt to the CTAs in equal consecutive runs, whatever
+// the lengths, by a prefix sum over the lengths that every warp does for itself; when items are
+// few, or their lengths near enough, each has CTAs of its own.  A run holds pieces of one or several
+// items; an item that lies in one run is written out directly, the pieces of one that does not go
+// to the workspace as fp32 O, max and sum, and the CTA that is last to finish (a counter that
+// wraps to zero) joins them in order, so the result does not depend on who that is.
 //
 // Inside a piece the warps take slices in turn, each with a softmax of its own (running max and sum,
 // O in registers) and a ring of its own in shared memory, filled by cp.async kStages - 1 slices
 // ahead, across piece borders: no barrier between warps until a piece ends and their parts are joined.
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = kDecodeWarps * 32;
-constexpr int kDecodeMaxCtas = 2 * 148;  // two per SM
-constexpr int kSlice = 16;               // keys
-constexpr int kRowsMax = 16;             // query heads of an item
+constexpr int kCtasPerSm = 3;            // of one block of query heads; two of two blocks
+constexpr int kDecodeMaxCtas = kCtasPerSm * 148;
+constexpr int kRowsMax = 16;             // query heads of an item, at most
 constexpr int kMinSlices = 16;           // fewest slices worth a CTA of their own
 constexpr int kAhead = 2;                // slices whose page ids are asked for before their load
 constexpr int kFewItems = 4;             // up to a quarter of the CTAs: a CTA per piece
-constexpr int kMergeCols = 32;           // columns of O joined at a time
-constexpr int kMergeStride = kMergeCols + 8;  // floats: 8 banks from row to row
+constexpr int kMergeCols = 32;           // columns of O in a strip of the merge buffer
+constexpr int kMergeStride = kMergeCols + 4;  // floats: two rows are 8 banks apart
+constexpr int kMergeSlots = 16;          // strips of a warp
+constexpr int kJoin = 8;                 // pieces read at a time in a join
+constexpr int kHeld = kDecodeWarps * kMergeStride;  // pieces whose weights fit in the merge buffer
 
-template <int D, bool kE4M3>
+template <int D, bool kE4M3, int R>
 struct DecodeCfg {
+    static constexpr int kRows = 8 * R;                     // query heads of an item
     static constexpr int kRowBytes = D * (kE4M3 ? 1 : 2);
+    // Keys of a slice: 16 of 256 bytes; 32 shorter ones, which leaves the chain of products, maxima and
+    // exponentials of a slice twice the bytes to hide behind
+    static constexpr int kSlice = kRowBytes >= 256 ? 16 : 32;
     static constexpr int kTileBytes = kSlice * kRowBytes;   // K or V of a slice
     static constexpr int kStageBytes = 2 * kTileBytes;
-    // 24 KB a warp: with two CTAs of four warps, 128 KB of loads in flight on the SM behind the
-    // slice that is being computed
-    static constexpr int kStages = kStageBytes >= 8192 ? 3 : kStageBytes >= 4096 ? 6 : 8;
+    static constexpr int kCtas = R == 1 ? kCtasPerSm : 2;
+    // 16 KB a warp with three CTAs of four warps on an SM, 24 KB with two: 96 or 128 KB of loads in flight
+    // behind the slices that are being computed
+    static constexpr int kStages = (R == 1 ? 16384 : 24576) / kStageBytes;
     static constexpr int kChunks = kRowBytes / 16;          // 16-byte chunks of a row
     static constexpr int kOffMerge = kDecodeWarps * kStages * kStageBytes;
-    static constexpr int kOffStats = kOffMerge + kDecodeWarps * kRowsMax * kMergeStride * 4;
+    static constexpr int kOffStats = kOffMerge + kDecodeWarps * kMergeSlots * kMergeStride * 4;
     static constexpr int kOffMask = kOffStats + 2 * kDecodeWarps * kRowsMax * 4;
-    static constexpr int kOffPlan = kOffMask + kDecodeWarps * kStages * 4;
-    static constexpr int kSmemBytes = kOffPlan + 64 + kDecodeWarps * 8;
-    static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
+    static constexpr int kOffLast = kOffMask + kDecodeWarps * kStages * 4;
+    static constexpr int kSmemBytes = kOffLast + 16;
+    static constexpr int kSlotFloats = kRows * D + 2 * kRows;  // a partial result
+    static_assert(kCtas * (kSmemBytes + 1024) <= 228 * 1024, "CTAs per SM");
 };
 
 // Chunk c of row r lies at chunk c ^ swizzle(r): eight consecutive rows then hold one chunk index in
 // different banks.
-template <int D, bool kE4M3>
+template <int kChunks>
 __device__ __forceinline__ int swizzle(int r) {
-    if constexpr (DecodeCfg<D, kE4M3>::kChunks == 4) return (r >> 1) & 3;
+    if constexpr (kChunks == 4) return (r >> 1) & 3;
     return r & 7;
 }
 
@@ -166,29 +178,42 @@ __device__ __forceinline__ void e4m3x4_to_half(uint32_t w, uint32_t& lo, uint32_
         : "=r"(lo), "=r"(hi)
         : "r"(w));
 }
+// An 8x8 matrix of 16-bit values across the warp, transposed.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__host__ __device__ constexpr int64_t run_start(int64_t cta, int64_t total, int64_t ctas) { return cta * total / ctas; }
-// The CTA whose run holds slice s.
-__device__ __forceinline__ int run_owner(int64_t s, int64_t total, int64_t ctas) {
-    return static_cast<int>(((s + 1) * ctas - 1) / total);
-}
+// Runs of `total` slices: the first `more` CTAs have one slice more than the others' `len`.
+struct Runs {
+    int len, more;
+    __device__ __forceinline__ int start(int cta) const { return cta * len + min(cta, more); }
+    // the CTA whose run holds slice s
+    __device__ __forceinline__ int owner(int s) const {
+        const int edge = more * (len + 1);
+        return s < edge ? static_cast<int>(static_cast<uint32_t>(s) / static_cast<uint32_t>(len + 1))
+                        : more + static_cast<int>(static_cast<uint32_t>(s - edge) / static_cast<uint32_t>(len));
+    }
+};
 
 // Walks a CTA's run piece by piece: slices [s0, s1) of item r of sequence b.
+template <int kSlice>
 struct RunCursor {
     int b, r, s0, s1;
-    int64_t left;  // slices of the run after this piece
+    int left;      // slices of the run after this piece
     Visible vis;
-    int n;         // slices of the item
+    int n;         // slices of the item: one at least, so that an empty one is written too
     __device__ __forceinline__ void enter(const DecodeArgs& a) {
         vis = visible_keys(a, __ldg(a.lens + b));
         n = max(1, (vis.count + kSlice - 1) / kSlice);
     }
     __device__ __forceinline__ void cut() {
-        s1 = static_cast<int>(min(static_cast<int64_t>(n), s0 + left));
+        s1 = min(n - s0, left) + s0;
         left -= s1 - s0;
     }
     __device__ __forceinline__ bool next(const DecodeArgs& a) {
@@ -204,15 +229,21 @@ struct RunCursor {
     }
 };
 
-template <int D, bool kE4M3>
-__global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const __grid_constant__ DecodeArgs a) {
-    using Cfg = DecodeCfg<D, kE4M3>;
+template <int D, bool kE4M3, int R>
+__global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
+    paged_decode_kernel(const __grid_constant__ DecodeArgs a) {
+    using Cfg = DecodeCfg<D, kE4M3, R>;
+    constexpr int kRows = Cfg::kRows;
     constexpr int kStages = Cfg::kStages;
-    constexpr int kSteps = D / 16;   // products of S per 8 keys
-    constexpr int kBlocks = D / 8;   // column blocks of O
-    // 8-bit path: weights as f16 times 2^15, which keeps 11 bits of every weight down to 2^-29 of the
-    // row's largest (and something down to 2^-39)
-    constexpr float kShift = kE4M3 ? 15.0f : 0.0f;
+    constexpr int kSlice = Cfg::kSlice;
+    constexpr int kChunks = Cfg::kChunks;
+    constexpr int kKb = kSlice / 16;  // blocks of 16 keys
+    constexpr int kSteps = D / 16;    // products of S per block; blocks of 16 columns of O
+    // The reference max moves only when a score passes it by more than 2^kLazy, so that most slices need
+    // one vote instead of a row maximum.  8-bit path: weights are f16 times 2^7, at most 2^15; all of
+    // their 11 bits are kept down to 2^-21 of the reference and something down to 2^-31.
+    constexpr float kLazy = 8.0f;
+    constexpr float kShift = kE4M3 ? 7.0f : 0.0f;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -221,113 +252,124 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
     float* stat_l = stat_m + kDecodeWarps * kRowsMax;
     uint32_t* masks = reinterpret_cast<uint32_t*>(smem + Cfg::kOffMask) + warp * kStages;
 
-    // ---- the run of this CTA
-    RunCursor cur;
-    int64_t total = 0, first = 0;  // slices of all items; this CTA's first one
-    int ctas = 0;
-    int few_piece = -1, few_pieces = 0;  // few items: which piece of its item this CTA has, of how many
+    // ---- the run of this CTA; every warp works it out for itself, a lane per batch / 32 sequences
+    RunCursor<kSlice> cur;
+    Runs runs{0, 0};
+    int first = 0;                   // number of this CTA's first slice
+    int few_piece = -1, pieces = 0;  // a CTA per piece: which piece of its item this one has, of how many
     {
-        int64_t* plan = reinterpret_cast<int64_t*>(smem + Cfg::kOffPlan);
-        int64_t* wsum = plan + 4;
-        const int per = (a.batch + kDecodeThreads - 1) / kDecodeThreads;
-        const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
-        // Sum of `mine` over all threads, and over those before this one.
-        auto scan = [&](int64_t mine, int64_t* before) {
-            int64_t incl = mine;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int64_t o = __shfl_up_sync(0xffffffffu, incl, off);
-                if (lane >= off) incl += o;
-            }
-            if (lane == 31) wsum[warp] = incl;
-            __syncthreads();
-            int64_t all = 0;
-            *before = incl - mine;
-#pragma unroll
-            for (int w = 0; w < kDecodeWarps; ++w) {
-                if (w < warp) *before += wsum[w];
-                all += wsum[w];
-            }
-            __syncthreads();
-            return all;
-        };
+        const int cta = static_cast<int>(blockIdx.x), grid = static_cast<int>(gridDim.x);
+        const int per = (a.batch + 31) / 32;
+        const int b0 = min(a.batch, lane * per), b1 = min(a.batch, b0 + per);
         auto slices_of = [&](int b) {
             const Visible v = visible_keys(a, __ldg(a.lens + b));
             return max(1, (v.count + kSlice - 1) / kSlice);
         };
-        int64_t mine = 0, before;
-        for (int b = b0; b < b1; ++b) mine += slices_of(b);
-        mine *= a.items_per_seq;
-        total = scan(mine, &before);
-        const int64_t items = static_cast<int64_t>(a.batch) * a.items_per_seq;
-        if (items * kFewItems <= gridDim.x) {
-            // few items: every piece has a CTA of its own, an item's pieces even
-            const int64_t room = gridDim.x - items;
-            const int64_t len = max(static_cast<int64_t>(kMinSlices), (total + room - 1) / room);
-            mine = 0;
-            for (int b = b0; b < b1; ++b) mine += (slices_of(b) + len - 1) / len * a.items_per_seq;
-            ctas = static_cast<int>(scan(mine, &before));
-            if (static_cast<int>(blockIdx.x) >= ctas) return;
-            if (static_cast<int>(blockIdx.x) >= before && static_cast<int>(blockIdx.x) < before + mine) {
-                for (int b = b0;; ++b) {
-                    const int pieces = static_cast<int>((slices_of(b) + len - 1) / len);
-                    const int64_t all = static_cast<int64_t>(pieces) * a.items_per_seq;
-                    if (blockIdx.x < before + all) {
-                        const int at = static_cast<int>(blockIdx.x - before);
-                        plan[0] = b;
-                        plan[1] = at / pieces;
-                        plan[2] = at % pieces;
-                        plan[3] = pieces;
-                        break;
-                    }
-                    before += all;
-                }
+        // sum over the lanes before this one; `all` of every lane
+        auto scan = [&](int mine, int& all) {
+            int incl = mine;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, incl, off);
+                if (lane >= off) incl += o;
             }
-            __syncthreads();
-            cur.b = static_cast<int>(plan[0]);
-            cur.r = static_cast<int>(plan[1]);
-            few_piece = static_cast<int>(plan[2]);
-            few_pieces = static_cast<int>(plan[3]);
-            cur.enter(a);
-            const int even = (cur.n + few_pieces - 1) / few_pieces;
-            cur.s0 = min(cur.n, few_piece * even);
-            cur.s1 = min(cur.n, cur.s0 + even);
-            cur.left = 0;
+            all = __shfl_sync(0xffffffffu, incl, 31);
+            return incl - mine;
+        };
+        int mine = 0, most = 0, total, before = 0;
+        if (a.batch == 1) {
+            most = slices_of(0);
+            total = most * a.items_per_seq;
+            mine = lane == 0 ? total : 0;
         } else {
-            const int64_t worth = (total + kMinSlices - 1) / kMinSlices;
-            ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), worth));
-            if (static_cast<int>(blockIdx.x) >= ctas) return;
-            first = run_start(blockIdx.x, total, ctas);
-            if (first >= before && first < before + mine) {
-                for (int b = b0;; ++b) {
-                    const int n = slices_of(b);
-                    const int64_t all = static_cast<int64_t>(n) * a.items_per_seq;
-                    if (first < before + all) {
-                        plan[0] = b;
-                        plan[1] = (first - before) / n;
-                        plan[2] = (first - before) % n;
+            for (int b = b0; b < b1; ++b) {
+                const int n = slices_of(b);
+                mine += n;
+                most = max(most, n);
+            }
+            most = __reduce_max_sync(0xffffffffu, most);
+            mine *= a.items_per_seq;
+            before = scan(mine, total);
+        }
+        const int items = a.batch * a.items_per_seq;
+        // A CTA per item when the longest is not much longer than an even share (about what streams in
+        // the time that cutting items and joining the pieces takes)
+        const bool whole_items = items <= grid && most <= total / 160 + 40;
+        const bool few = whole_items || items <= grid / kFewItems;
+        int at_b = 0, at_r = 0, at_s = 0;
+        if (whole_items) {
+            if (cta >= items) return;
+            at_b = static_cast<int>(fast_div(static_cast<uint32_t>(cta), a.fd_items));
+            at_r = cta - at_b * a.items_per_seq;
+            pieces = 1;
+        } else {
+            int len = 1;  // few items: slices of a piece, at most
+            if (few) {
+                // an item's pieces are even, and their weights fit the merge buffer
+                len = max(max(kMinSlices, total / (grid - items) + 1), (most + kHeld - 1) / kHeld);
+                if (a.batch == 1) {
+                    total = (most + len - 1) / len * a.items_per_seq;
+                    mine = lane == 0 ? total : 0;
+                } else {
+                    mine = 0;
+                    for (int b = b0; b < b1; ++b) mine += (slices_of(b) + len - 1) / len * a.items_per_seq;
+                    before = scan(mine, total);
+                }
+                if (cta >= total) return;
+                first = cta;
+            } else {
+                const int ctas = min(grid, (total + kMinSlices - 1) / kMinSlices);
+                if (cta >= ctas) return;
+                runs.len = total / ctas;
+                runs.more = total - runs.len * ctas;
+                first = runs.start(cta);
+            }
+            // the lane whose sequences hold `first` finds the item and the slice (or piece) in it
+            const bool here = first >= before && first < before + mine;
+            if (here) {
+                for (at_b = b0;; ++at_b) {
+                    const int n = (slices_of(at_b) + len - 1) / len;
+                    if (first < before + n * a.items_per_seq) {
+                        at_r = static_cast<int>(static_cast<uint32_t>(first - before) / static_cast<uint32_t>(n));
+                        at_s = first - before - at_r * n;
                         break;
                     }
-                    before += all;
+                    before += n * a.items_per_seq;
                 }
             }
-            __syncthreads();
-            cur.b = static_cast<int>(plan[0]);
-            cur.r = static_cast<int>(plan[1]);
-            cur.s0 = static_cast<int>(plan[2]);
-            cur.left = run_start(blockIdx.x + 1, total, ctas) - first;
-            cur.enter(a);
+            const int who = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+            at_b = __shfl_sync(0xffffffffu, at_b, who);
+            at_r = __shfl_sync(0xffffffffu, at_r, who);
+            at_s = __shfl_sync(0xffffffffu, at_s, who);
+            pieces = len;
+        }
+        cur.b = at_b;
+        cur.r = at_r;
+        cur.s0 = at_s;
+        cur.enter(a);
+        if (few) {
+            few_piece = at_s;
+            cur.s1 = cur.n;
+            cur.left = 0;
+            if (!whole_items) {
+                pieces = (cur.n + pieces - 1) / pieces;
+                const int even = (cur.n + pieces - 1) / pieces;
+                cur.s0 = min(cur.n, few_piece * even);
+                cur.s1 = min(cur.n, cur.s0 + even);
+            }
+        } else {
+            cur.left = runs.start(cta + 1) - first;
             cur.cut();
         }
     }
 
     // ---- loads: this warp's slices s0 + warp, s0 + warp + 4, ... of every piece, in order
     const uint32_t ring = ptx::smem_u32(smem) + warp * (kStages * Cfg::kStageBytes);
-    RunCursor ld = cur;
+    RunCursor<kSlice> ld = cur;
     int ld_s = ld.s0 + warp;
     int ld_slot = 0;  // ring slot of the next load
-    // The slices after the next load, whose page ids are on their way: lanes 0-15 stand for the keys' K
-    // rows, 16-31 for their V rows.  slot_in_page -1: key not seen; head -1: no slice left.
+    // The slices after the next load, whose page ids are on their way; a lane stands for the key
+    // lane % kSlice.  slot_in_page -1: key not seen; head -1: no slice left.
     int page[kAhead], slot_in_page[kAhead], head[kAhead];
     auto seek = [&](int i) {
         head[i] = -1;
@@ -336,7 +378,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
             ld_s = ld.s0 + warp;
         }
         head[i] = ld.r / a.row_tiles;
-        const int u = ld_s * kSlice + (lane & 15);
+        const int u = ld_s * kSlice + lane % kSlice;
         slot_in_page[i] = -1;
         if (u < ld.vis.count) {
             const int j = ld.vis.key(u);
@@ -346,31 +388,36 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
         }
         ld_s += kDecodeWarps;
     };
+    constexpr uint32_t kNoRow = 0xffffffffu;
+    const int chunk = lane % kChunks;
     auto load = [&]() {
         if (head[0] >= 0) {
-            int64_t off = -1;
+            // rows in 16-byte units (the host refuses caches past 64 GB)
+            uint32_t k_off = kNoRow, v_off = kNoRow;
             if (slot_in_page[0] >= 0) {
-                if (page[0] < 0 || page[0] >= a.c.num_pages)
+                if (page[0] < 0 || page[0] >= a.c.num_pages) {
                     bad_page(a.c);
-                else if (lane < 16)
-                    off = page[0] * a.c.k_page + head[0] * a.c.k_head + slot_in_page[0] * a.c.k_slot;
-                else
-                    off = page[0] * a.c.v_page + head[0] * a.c.v_head + slot_in_page[0] * a.c.v_slot;
+                } else {
+                    k_off = static_cast<uint32_t>(page[0]) * a.k16_page + static_cast<uint32_t>(head[0]) * a.k16_head +
+                            static_cast<uint32_t>(slot_in_page[0]) * a.k16_slot;
+                    v_off = static_cast<uint32_t>(page[0]) * a.v16_page + static_cast<uint32_t>(head[0]) * a.v16_head +
+                            static_cast<uint32_t>(slot_in_page[0]) * a.v16_slot;
+                }
             }
-            const uint32_t seen = __ballot_sync(0xffffffffu, off >= 0);
-            if (lane == 0) masks[ld_slot] = seen & 0xffffu;
-            constexpr int kRowsPer = 32 / Cfg::kChunks;  // rows per instruction
-            const int c = lane % Cfg::kChunks;
+            const uint32_t seen = __ballot_sync(0xffffffffu, k_off != kNoRow);
+            if (lane == 0) masks[ld_slot] = seen;
+            constexpr int kRowsPer = 32 / kChunks;  // rows per instruction
             const uint32_t dst = ring + ld_slot * Cfg::kStageBytes;
 #pragma unroll
             for (int i = 0; i < kSlice / kRowsPer; ++i) {
-                const int row = i * kRowsPer + lane / Cfg::kChunks;
-                const uint32_t at = dst + row * Cfg::kRowBytes + ((c ^ swizzle<D, kE4M3>(row)) << 4);
-                const int64_t ko = __shfl_sync(0xffffffffu, off, row);
-                const int64_t vo = __shfl_sync(0xffffffffu, off, 16 + row);
+                const int row = i * kRowsPer + lane / kChunks;
+                const uint32_t at = dst + row * Cfg::kRowBytes + ((chunk ^ swizzle<kChunks>(row)) << 4);
+                const uint32_t ko = __shfl_sync(0xffffffffu, k_off, row);
+                const uint32_t vo = __shfl_sync(0xffffffffu, v_off, row);
                 // rows that are not seen read as zeros (their bytes are not touched)
-                cp_async16(at, a.c.k + (ko < 0 ? 0 : ko + c * 16), ko < 0 ? 0 : 16);
-                cp_async16(at + Cfg::kTileBytes, a.c.v + (vo < 0 ? 0 : vo + c * 16), vo < 0 ? 0 : 16);
+                const int bytes = ko == kNoRow ? 0 : 16;
+                cp_async16(at, a.c.k + (static_cast<uint64_t>(bytes ? ko + chunk : 0) << 4), bytes);
+                cp_async16(at + Cfg::kTileBytes, a.c.v + (static_cast<uint64_t>(bytes ? vo + chunk : 0) << 4), bytes);
             }
             ld_slot = ld_slot + 1 == kStages ? 0 : ld_slot + 1;
 #pragma unroll
@@ -385,32 +432,33 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
     };
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) seek(i);
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < kStages - 1; ++i) load();
 
     int slot = 0;  // ring slot of the next slice to compute
-    int64_t item0 = first - cur.s0;  // slice number, over all items, of the item's first
+    int item0 = first - cur.s0;  // number of the item's first slice
     for (;;) {
         const int hk = cur.r / a.row_tiles;
-        const int row0 = (cur.r - hk * a.row_tiles) * kRowsMax;  // first query head of the item, within the group
-        const int rows = min(kRowsMax, a.group - row0);
+        const int row0 = (cur.r - hk * a.row_tiles) * kRows;  // first query head of the item, within the group
+        const int rows = min(kRows, a.group - row0);
         const int h0 = hk * a.group + row0;
 
-        // ---- Q as the A operand of S = Q K^T: rows g and g + 8
-        uint32_t qf[kSteps][4];
-        float unit[2] = {1.0f, 1.0f};  // 8-bit path: what one unit of S is worth, by row
+        // ---- Q as the B operand of S^T = K Q^T: query head g of each block
+        uint32_t qf[R][kSteps][2];
+        float unit[R];  // 8-bit path: what one unit of S is worth, for query head g of the block
         {
             const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + cur.b * a.q_b + h0 * a.q_h;
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int row = g + 8 * hf;
+            for (int rb = 0; rb < R; ++rb) {
+                const int row = g + 8 * rb;
                 const bool ok = row < rows;
                 const __nv_bfloat16* qr = q + (ok ? row : 0) * a.q_h;
+                unit[rb] = 1.0f;
                 if constexpr (!kE4M3) {
 #pragma unroll
                     for (int kk = 0; kk < kSteps; ++kk) {
-                        qf[kk][hf] = ok ? __ldg(reinterpret_cast<const uint32_t*>(qr + kk * 16 + 2 * t)) : 0u;
-                        qf[kk][2 + hf] = ok ? __ldg(reinterpret_cast<const uint32_t*>(qr + kk * 16 + 8 + 2 * t)) : 0u;
+                        qf[rb][kk][0] = ok ? __ldg(reinterpret_cast<const uint32_t*>(qr + kk * 16 + 2 * t)) : 0u;
+                        qf[rb][kk][1] = ok ? __ldg(reinterpret_cast<const uint32_t*>(qr + kk * 16 + 8 + 2 * t)) : 0u;
                     }
                 } else {
                     // lane t holds the D/4 consecutive features whose 8-bit keys it reads; as f16, scaled
@@ -429,40 +477,46 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
                     int e = static_cast<int>(__float_as_uint(mx) >> 23) - 127;
                     e = mx == 0.0f || e > 127 ? 14 : max(e, -100);
                     const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
-                    unit[hf] = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+                    unit[rb] = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
 #pragma unroll
                     for (int kk = 0; kk < kSteps; ++kk) {
-                        qf[kk][hf] = pack_half2(__uint_as_float(w[kk].x << 16) * up, __uint_as_float(w[kk].x & 0xFFFF0000u) * up);
-                        qf[kk][2 + hf] = pack_half2(__uint_as_float(w[kk].y << 16) * up, __uint_as_float(w[kk].y & 0xFFFF0000u) * up);
+                        qf[rb][kk][0] = pack_half2(__uint_as_float(w[kk].x << 16) * up, __uint_as_float(w[kk].x & 0xFFFF0000u) * up);
+                        qf[rb][kk][1] = pack_half2(__uint_as_float(w[kk].y << 16) * up, __uint_as_float(w[kk].y & 0xFFFF0000u) * up);
                     }
                 }
             }
         }
-        float slope[2] = {0.0f, 0.0f};
-        if (a.has_alibi) {
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int h = h0 + g + 8 * hf;
-                if (g + 8 * hf < rows)
-                    slope[hf] = a.alibi_generated ? exp2f(-8.0f * static_cast<float>(h + 1) / static_cast<float>(a.heads_q))
-                                                  : a.alibi_slopes[h];
-            }
-        }
         const float ks = a.c.k_scale ? __ldg(a.c.k_scale + hk) : 1.0f;
         const bool capped = a.softcap > 0.0f;
-        // score = S * mul + slope * (j - p): log2 units, or units of the soft-cap
+        // score = S * mul + slope * (j - p), in log2 units or in units of the soft-cap; a thread has
+        // query heads 2t, 2t + 1 of each block
         const float into = capped ? a.inv_softcap : kLog2e;
-        float mul[2];
+        float mul[2 * R], slope[2 * R];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            mul[hf] = a.scale * unit[hf] * ks * into;
-            slope[hf] *= into;
+        for (int i = 0; i < 2 * R; ++i) {
+            const int row = 2 * t + (i & 1) + 8 * (i >> 1);
+            const float u = kE4M3 ? __shfl_sync(0xffffffffu, unit[i >> 1], 4 * (2 * t + (i & 1))) : 1.0f;
+            mul[i] = a.scale * u * ks * into;
+            slope[i] = 0.0f;
+            if (a.has_alibi && row < rows) {
+                const int h = h0 + row;
+                slope[i] = into * (a.alibi_generated ? exp2f(-8.0f * static_cast<float>(h + 1) / static_cast<float>(a.heads_q))
+                                                     : a.alibi_slopes[h]);
+            }
         }
 
-        float o[kBlocks][4];
+        // O^T: block j of 16 columns by query heads 2t, 2t + 1 of block rb
+        float o[R][kSteps][4];
 #pragma unroll
-        for (int j = 0; j < kBlocks; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        for (int rb = 0; rb < R; ++rb)
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) o[rb][j][0] = o[rb][j][1] = o[rb][j][2] = o[rb][j][3] = 0.0f;
+        float m[2 * R], l[2 * R];
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+        }
 
         for (int s = cur.s0 + warp; s < cur.s1; s += kDecodeWarps) {
             cp_async_wait<kStages - 2>();
@@ -473,146 +527,181 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
             const uint32_t seen = masks[slot];
             slot = slot + 1 == kStages ? 0 : slot + 1;
 
-            // S[16 rows x 16 keys]: keys 2t, 2t + 1 of the lower and the upper eight
-            float sc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-            if constexpr (!kE4M3) {
-                const int key = ((lane >> 4) << 3) + (lane & 7);
-                const uint32_t at = kt + key * Cfg::kRowBytes + ((((lane >> 3) & 1) ^ swizzle<D, kE4M3>(key)) << 4);
+            // S^T: keys g, g + 8 of each block of 16 by query heads 2t, 2t + 1; the steps of a block sum
+            // in kChains chains, so that four or more are under way
+            constexpr int kChains = kKb * R >= 4 ? 1 : 4 / (kKb * R);
+            float sc[kKb][R][4], chain[kChains][kKb][R][4];
 #pragma unroll
-                for (int kk = 0; kk < kSteps; ++kk) {
-                    uint32_t b[4];
-                    ldmatrix4(at ^ (kk << 5), b);
-                    mma16816<false>(sc[0], qf[kk], b[0], b[1]);
-                    mma16816<false>(sc[1], qf[kk], b[2], b[3]);
-                }
-            } else {
+            for (int c = 0; c < kChains; ++c)
 #pragma unroll
-                for (int nb = 0; nb < 2; ++nb) {
-                    const int key = nb * 8 + g;
+                for (int kb = 0; kb < kKb; ++kb)
+#pragma unroll
+                    for (int rb = 0; rb < R; ++rb)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) chain[c][kb][rb][i] = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < kKb; ++kb) {
+                if constexpr (!kE4M3) {
+                    const int key = kb * 16 + (lane & 15);
+                    const uint32_t at = kt + key * Cfg::kRowBytes + (((lane >> 4) ^ swizzle<kChunks>(key)) << 4);
+#pragma unroll
+                    for (int kk = 0; kk < kSteps; ++kk) {
+                        uint32_t k[4];
+                        ldmatrix4(at ^ (kk << 5), k);
+#pragma unroll
+                        for (int rb = 0; rb < R; ++rb)
+                            mma16816<false>(chain[kk % kChains][kb][rb], k, qf[rb][kk][0], qf[rb][kk][1]);
+                    }
+                } else {
+                    const int key = kb * 16 + g;
 #pragma unroll
                     for (int c = 0; c < kSteps / 4; ++c) {
-                        const int chunk = (kSteps / 4) * t + c;
-                        const uint4 w = lds128(kt + key * Cfg::kRowBytes + ((chunk ^ swizzle<D, kE4M3>(key)) << 4));
-                        uint32_t b0, b1;
-                        e4m3x4_to_half(w.x, b0, b1);
-                        mma16816<true>(sc[nb], qf[4 * c + 0], b0, b1);
-                        e4m3x4_to_half(w.y, b0, b1);
-                        mma16816<true>(sc[nb], qf[4 * c + 1], b0, b1);
-                        e4m3x4_to_half(w.z, b0, b1);
-                        mma16816<true>(sc[nb], qf[4 * c + 2], b0, b1);
-                        e4m3x4_to_half(w.w, b0, b1);
-                        mma16816<true>(sc[nb], qf[4 * c + 3], b0, b1);
+                        const int ch = (kSteps / 4) * t + c;
+                        const uint4 w0 = lds128(kt + key * Cfg::kRowBytes + ((ch ^ swizzle<kChunks>(key)) << 4));
+                        const uint4 w1 = lds128(kt + (key + 8) * Cfg::kRowBytes + ((ch ^ swizzle<kChunks>(key + 8)) << 4));
+                        const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t k[4];
+                            e4m3x4_to_half(x0[i], k[0], k[2]);
+                            e4m3x4_to_half(x1[i], k[1], k[3]);
+#pragma unroll
+                            for (int rb = 0; rb < R; ++rb)
+                                mma16816<true>(chain[i % kChains][kb][rb], k, qf[rb][4 * c + i][0], qf[rb][4 * c + i][1]);
+                        }
                     }
                 }
             }
 
-            // score mods, mask, running max
-            float mx[2] = {-INFINITY, -INFINITY};
+            // score mods, mask, and whether a score passes the reference max
+            float mx[2 * R];
 #pragma unroll
-            for (int nb = 0; nb < 2; ++nb) {
+            for (int i = 0; i < 2 * R; ++i) mx[i] = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = nb * 8 + 2 * t + (i & 1);
-                    float x = sc[nb][i] * mul[i >> 1];
-                    if (a.has_alibi)
-                        x += slope[i >> 1] * static_cast<float>(cur.vis.key(s * kSlice + key) - (cur.vis.len - 1));
-                    if (capped) x = a.softcap * kLog2e * tanhf(x);
-                    x = (seen >> key) & 1u ? x : -INFINITY;
-                    sc[nb][i] = x;
-                    mx[i >> 1] = fmaxf(mx[i >> 1], x);
-                }
-            }
-            bool moved = false;
-            float alpha[2];
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
-                mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
-                const float mn = fmaxf(m[hf], mx[hf]);
-                alpha[hf] = mn > m[hf] ? ptx::ex2(m[hf] - mn) : 1.0f;
-                moved |= mn > m[hf];
-                m[hf] = mn;
-            }
-            if (__any_sync(0xffffffffu, moved)) {
-                l[0] *= alpha[0];
-                l[1] *= alpha[1];
-#pragma unroll
-                for (int j = 0; j < kBlocks; ++j) {
-                    o[j][0] *= alpha[0];
-                    o[j][1] *= alpha[0];
-                    o[j][2] *= alpha[1];
-                    o[j][3] *= alpha[1];
-                }
-            }
-            const float ref[2] = {(m[0] == -INFINITY ? 0.0f : m[0]) - kShift, (m[1] == -INFINITY ? 0.0f : m[1]) - kShift};
-            // P in the operand's type; l sums it before that rounding
-            uint32_t p[4];
-#pragma unroll
-            for (int nb = 0; nb < 2; ++nb) {
-                float e[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) e[i] = ptx::ex2(sc[nb][i] - ref[i >> 1]);
-                l[0] += e[0] + e[1];
-                l[1] += e[2] + e[3];
-                p[2 * nb] = kE4M3 ? pack_half2(e[0], e[1]) : ptx::pack_bf16x2(e[0], e[1]);
-                p[2 * nb + 1] = kE4M3 ? pack_half2(e[2], e[3]) : ptx::pack_bf16x2(e[2], e[3]);
-            }
-
-            // O += P V
-            if constexpr (!kE4M3) {
-                const int key = (((lane >> 3) & 1) << 3) + (lane & 7);
-                const uint32_t at = vt + key * Cfg::kRowBytes + (((lane >> 4) ^ swizzle<D, kE4M3>(key)) << 4);
-#pragma unroll
-                for (int dd = 0; dd < kSteps; ++dd) {
-                    uint32_t b[4];
-                    ldmatrix4_trans(at ^ (dd << 5), b);
-                    mma16816<false>(o[2 * dd], p, b[0], b[1]);
-                    mma16816<false>(o[2 * dd + 1], p, b[2], b[3]);
-                }
-            } else {
-                // column n of block j is feature (D/8) n + j: lane g reads D/8 consecutive features of
-                // keys 2t, 2t+1, 2t+8, 2t+9 and pairs the keys' bytes feature by feature
-                uint32_t w[4][D / 32];
+            for (int kb = 0; kb < kKb; ++kb) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int key = 2 * t + (i & 1) + 8 * (i >> 1);
-                    if constexpr (D == 128) {
-                        const uint4 x = lds128(vt + key * Cfg::kRowBytes + ((g ^ swizzle<D, kE4M3>(key)) << 4));
-                        w[i][0] = x.x;
-                        w[i][1] = x.y;
-                        w[i][2] = x.z;
-                        w[i][3] = x.w;
-                    } else {
-                        const uint2 x = lds64(vt + key * Cfg::kRowBytes + (((g >> 1) ^ swizzle<D, kE4M3>(key)) << 4) + (g & 1) * 8);
-                        w[i][0] = x.x;
-                        w[i][1] = x.y;
+                    const int key = kb * 16 + g + 8 * (i >> 1);
+                    const bool on = (seen >> key) & 1u;
+#pragma unroll
+                    for (int rb = 0; rb < R; ++rb) {
+                        const int h = 2 * rb + (i & 1);
+                        float x = chain[0][kb][rb][i];
+#pragma unroll
+                        for (int c = 1; c < kChains; ++c) x += chain[c][kb][rb][i];
+                        x *= mul[h];
+                        if (a.has_alibi) x += slope[h] * static_cast<float>(cur.vis.key(s * kSlice + key) - (cur.vis.len - 1));
+                        if (capped) x = a.softcap * kLog2e * tanhf(x);
+                        x = on ? x : -INFINITY;
+                        sc[kb][rb][i] = x;
+                        mx[h] = fmaxf(mx[h], x);
                     }
                 }
+            }
+            bool passes = false;
 #pragma unroll
-                for (int q4 = 0; q4 < D / 32; ++q4) {
-                    uint32_t b0[4], b1[4];
-                    e4m3x4_to_half(__byte_perm(w[0][q4], w[1][q4], 0x5140), b0[0], b0[1]);
-                    e4m3x4_to_half(__byte_perm(w[0][q4], w[1][q4], 0x7362), b0[2], b0[3]);
-                    e4m3x4_to_half(__byte_perm(w[2][q4], w[3][q4], 0x5140), b1[0], b1[1]);
-                    e4m3x4_to_half(__byte_perm(w[2][q4], w[3][q4], 0x7362), b1[2], b1[3]);
+            for (int i = 0; i < 2 * R; ++i) passes |= mx[i] > m[i] + kLazy;
+            if (__any_sync(0xffffffffu, passes)) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mma16816<true>(o[4 * q4 + i], p, b0[i], b1[i]);
+                for (int i = 0; i < 2 * R; ++i) {
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], off));
+                    float alpha = 1.0f;
+                    if (mx[i] > m[i]) {
+                        alpha = ptx::ex2(m[i] - mx[i]);
+                        m[i] = mx[i];
+                    }
+                    l[i] *= alpha;
+#pragma unroll
+                    for (int j = 0; j < kSteps; ++j) {
+                        o[i >> 1][j][i & 1] *= alpha;
+                        o[i >> 1][j][2 + (i & 1)] *= alpha;
+                    }
+                }
+            }
+            float ref[2 * R];
+#pragma unroll
+            for (int i = 0; i < 2 * R; ++i) ref[i] = (m[i] == -INFINITY ? 0.0f : m[i]) - kShift;
+            // P in the operand's type, transposed to keys 2t, 2t + 1 by query head g; l sums it before that
+            // rounding
+            uint32_t p[kKb][R][2];
+#pragma unroll
+            for (int kb = 0; kb < kKb; ++kb) {
+#pragma unroll
+                for (int rb = 0; rb < R; ++rb) {
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const float e0 = ptx::ex2(sc[kb][rb][2 * hf] - ref[2 * rb]);
+                        const float e1 = ptx::ex2(sc[kb][rb][2 * hf + 1] - ref[2 * rb + 1]);
+                        l[2 * rb] += e0;
+                        l[2 * rb + 1] += e1;
+                        p[kb][rb][hf] = movmatrix_trans(kE4M3 ? pack_half2(e0, e1) : ptx::pack_bf16x2(e0, e1));
+                    }
+                }
+            }
+
+            // O^T += V^T P^T
+#pragma unroll
+            for (int kb = 0; kb < kKb; ++kb) {
+                if constexpr (!kE4M3) {
+                    const int key = kb * 16 + ((lane >> 4) << 3) + (lane & 7);
+                    const uint32_t at = vt + key * Cfg::kRowBytes + ((((lane >> 3) & 1) ^ swizzle<kChunks>(key)) << 4);
+#pragma unroll
+                    for (int j = 0; j < kSteps; ++j) {
+                        uint32_t v[4];
+                        ldmatrix4_trans(at ^ (j << 5), v);
+#pragma unroll
+                        for (int rb = 0; rb < R; ++rb) mma16816<false>(o[rb][j], v, p[kb][rb][0], p[kb][rb][1]);
+                    }
+                } else {
+                    // rows g and g + 8 of block j are columns (D/8) g + 2j and + 1: lane g reads D/8 consecutive
+                    // ones of keys 2t, 2t+1, 2t+8, 2t+9 and pairs the keys' bytes column by column
+                    uint32_t w[4][D / 32];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = kb * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
+                        if constexpr (D == 128) {
+                            const uint4 x = lds128(vt + key * Cfg::kRowBytes + ((g ^ swizzle<kChunks>(key)) << 4));
+                            w[i][0] = x.x;
+                            w[i][1] = x.y;
+                            w[i][2] = x.z;
+                            w[i][3] = x.w;
+                        } else {
+                            const uint2 x =
+                                lds64(vt + key * Cfg::kRowBytes + (((g >> 1) ^ swizzle<kChunks>(key)) << 4) + (g & 1) * 8);
+                            w[i][0] = x.x;
+                            w[i][1] = x.y;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < kSteps; ++j) {
+                        uint32_t v[4];
+                        const uint32_t sel = j & 1 ? 0x7362 : 0x5140;
+                        e4m3x4_to_half(__byte_perm(w[0][j >> 1], w[1][j >> 1], sel), v[0], v[1]);
+                        e4m3x4_to_half(__byte_perm(w[2][j >> 1], w[3][j >> 1], sel), v[2], v[3]);
+#pragma unroll
+                        for (int rb = 0; rb < R; ++rb) mma16816<true>(o[rb][j], v, p[kb][rb][0], p[kb][rb][1]);
+                    }
                 }
             }
         }
 
         // ---- the warps' parts of the piece: a common max, then O in strips of kMergeCols columns
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
-            l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
-            if (t == 0) {
-                stat_m[warp * kRowsMax + g + 8 * hf] = m[hf];
-                stat_l[warp * kRowsMax + g + 8 * hf] = l[hf];
+        for (int i = 0; i < 2 * R; ++i) {
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
+            if (g == 0) {
+                const int row = 2 * t + (i & 1) + 8 * (i >> 1);
+                stat_m[warp * kRowsMax + row] = m[i];
+                stat_l[warp * kRowsMax + row] = l[i];
             }
         }
         __syncthreads();
-        const int row = threadIdx.x >> 3;  // of the joined result: 16 rows x 8 threads of 4 columns
+        // a thread's place in the joined strips: 16 slots x 8 threads of 4 columns; a slot is a query head, with
+        // one block of them in one of two strips
+        const int strip_of = R == 1 ? threadIdx.x >> 6 : 0;
+        const int row = (threadIdx.x >> 3) & (kRows - 1);
         const bool row_ok = row < rows;
         float M = -INFINITY, L = 0.0f, wt[kDecodeWarps];
 #pragma unroll
@@ -626,7 +715,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
         const bool whole = cur.s0 == 0 && cur.s1 == cur.n;
         // partial results: slot 2c + 1 for the item that starts in this run, 2c for one that started before
         float* slots = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + kDecodeCounterBytes);
-        constexpr int kSlotFloats = kRowsMax * D + 2 * kRowsMax;
+        constexpr int kSlotFloats = Cfg::kSlotFloats;
         float* part = slots + (2 * static_cast<int64_t>(blockIdx.x) + (cur.s0 == 0 ? 1 : 0)) * kSlotFloats;
         const float vs = a.c.v_scale ? __ldg(a.c.v_scale + hk) : 1.0f;
         auto write_out = [&](int r, int col, float4 x, float sum) {
@@ -644,63 +733,68 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
                 a.lse[static_cast<int64_t>(cur.b) * a.heads_q + h0 + r] =
                     sum == 0.0f ? -INFINITY : (mr + (log2f(sum) - kShift)) * kLn2;
         };
-        // A strip is four column blocks: bf16 columns 8 j + n, in order; 8-bit features (D/8) n + j, four
-        // in a row for each n.  With at most 8 rows the other half of the buffer takes every second strip.
-        const int other = rows <= 8 ? 8 * kMergeStride : 0;
+        // A strip is two blocks of 16 columns: in order in a bf16 cache; columns (D/8) g + 4 strip .. + 3 for
+        // each g in an 8-bit one.
+        constexpr int kPass = 2 / R;  // strips at a time
 #pragma unroll
-        for (int q4 = 0; q4 < kBlocks / 4; ++q4) {
-            float* buf = merge + ((q4 & 1) ? other : 0);
-            if (q4 > 0 && other == 0) __syncthreads();  // the strip before has been read
+        for (int q0 = 0; q0 < D / kMergeCols; q0 += kPass) {
+            if (q0 > 0) __syncthreads();  // the strips before have been read
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int r = g + 8 * hf;
-                float* dst = buf + (warp * kRowsMax + r) * kMergeStride;
-                if (r < rows) {
+            for (int qq = 0; qq < kPass; ++qq) {
+#pragma unroll
+                for (int i = 0; i < 2 * R; ++i) {
+                    const int r = 2 * t + (i & 1) + 8 * (i >> 1);
+                    const int j = 2 * (q0 + qq);
+                    float* dst = merge + (warp * kMergeSlots + 8 * qq + r) * kMergeStride;
+                    const float x0 = o[i >> 1][j][i & 1], x1 = o[i >> 1][j][2 + (i & 1)];
+                    const float x2 = o[i >> 1][j + 1][i & 1], x3 = o[i >> 1][j + 1][2 + (i & 1)];
                     if constexpr (kE4M3) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            *reinterpret_cast<float4*>(dst + (2 * t + i) * 4) =
-                                make_float4(o[4 * q4][2 * hf + i], o[4 * q4 + 1][2 * hf + i], o[4 * q4 + 2][2 * hf + i],
-                                            o[4 * q4 + 3][2 * hf + i]);
+                        *reinterpret_cast<float4*>(dst + 4 * g) = make_float4(x0, x1, x2, x3);
                     } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            *reinterpret_cast<float2*>(dst + 8 * j + 2 * t) = make_float2(o[4 * q4 + j][2 * hf], o[4 * q4 + j][2 * hf + 1]);
+                        dst[g] = x0;
+                        dst[g + 8] = x1;
+                        dst[g + 16] = x2;
+                        dst[g + 24] = x3;
                     }
                 }
             }
             __syncthreads();
             if (row_ok) {
                 const int c4 = threadIdx.x & 7;
+                const int strip = q0 + strip_of;
                 float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int w = 0; w < kDecodeWarps; ++w) {
-                    const float4 y = *reinterpret_cast<const float4*>(buf + (w * kRowsMax + row) * kMergeStride + 4 * c4);
+                    const float4 y = *reinterpret_cast<const float4*>(
+                        merge + (w * kMergeSlots + (threadIdx.x >> 3)) * kMergeStride + 4 * c4);
                     x.x += wt[w] * y.x;
                     x.y += wt[w] * y.y;
                     x.z += wt[w] * y.z;
                     x.w += wt[w] * y.w;
                 }
-                const int d = kE4M3 ? (D / 8) * c4 + 4 * q4 : kMergeCols * q4 + 4 * c4;
+                const int d = kE4M3 ? (D / 8) * c4 + 4 * strip : kMergeCols * strip + 4 * c4;
                 if (whole)
                     write_out(row, d, x, L);
                 else
                     *reinterpret_cast<float4*>(part + row * D + d) = x;
             }
         }
-        if (row_ok && (threadIdx.x & 7) == 0) {
+        if (row_ok && strip_of == 0 && (threadIdx.x & 7) == 0) {
             if (whole) {
                 write_lse(row, M, L);
             } else {
-                part[kRowsMax * D + row] = M;
-                part[kRowsMax * D + kRowsMax + row] = L;
+                part[kRows * D + row] = M;
+                part[kRows * D + kRows + row] = L;
             }
         }
         if (!whole) {
-            const int c_first = few_piece >= 0 ? static_cast<int>(blockIdx.x) - few_piece : run_owner(item0, total, ctas);
-            const int pieces = few_piece >= 0 ? few_pieces : run_owner(item0 + cur.n - 1, total, ctas) - c_first + 1;
+            int c_first = static_cast<int>(blockIdx.x) - few_piece;
+            if (few_piece < 0) {
+                c_first = runs.owner(item0);
+                pieces = runs.owner(item0 + cur.n - 1) - c_first + 1;
+            }
             __syncthreads();  // the CTA's part is written, as seen from its first thread
-            int* last = reinterpret_cast<int*>(smem + Cfg::kOffPlan);
+            int* last = reinterpret_cast<int*>(smem + Cfg::kOffLast);
             if (threadIdx.x == 0) {
                 __threadfence();
                 const unsigned int old =
@@ -709,100 +803,106 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) paged_decode_kernel(const _
                 *last = old == static_cast<unsigned int>(pieces - 1);
             }
             __syncthreads();
-            const bool join = *last != 0;
-            __syncthreads();
-            if (join) {
-                auto piece = [&](int k) {
-                    return slots + (2 * static_cast<int64_t>(c_first + k) + (k == 0 ? 1 : 0)) * kSlotFloats;
-                };
-                // the pieces' weights by row (8 threads to a row), then O, float4 units of the rows spread
-                // over the threads (with few rows, the pieces too) so that many loads are in flight
-                constexpr int kHeld = kDecodeWarps * kMergeStride;
-                float* wts = merge;  // [min(pieces, kHeld)][kRowsMax]
-                float mj = -INFINITY, lj = 0.0f;
-#pragma unroll 4
-                for (int k = threadIdx.x & 7; k < pieces; k += 8) {
-                    const float mk = __ldcg(piece(k) + kRowsMax * D + row);
-                    const float lk = __ldcg(piece(k) + kRowsMax * D + kRowsMax + row);
-                    if (k < kHeld) wts[k * kRowsMax + row] = mk;
-                    const float mn = fmaxf(mj, mk);
-                    if (mn != -INFINITY) lj = lj * ptx::ex2(mj - mn) + lk * ptx::ex2(mk - mn);
-                    else lj += lk;  // 0, or NaN
-                    mj = mn;
-                }
+            if (*last != 0) {
+                // Every step here waits for L2 (about 0.5 us) and comes from a cold instruction cache, so: few
+                // steps, many loads to a step, little code.
+                const float* p0 = slots + 2 * static_cast<int64_t>(c_first) * kSlotFloats;  // piece k > 0: 2 k slots on
+                auto piece = [&](int k) { return p0 + (k == 0 ? kSlotFloats : 2 * k * kSlotFloats); };
+                auto weight = [](float mk, float mr) { return mk == -INFINITY ? 0.0f : ptx::ex2(mk - mr); };
+                float* wts = merge;  // [kHeld][kRowsMax]
+                // common max and sum, a warp to a row
+#pragma unroll 2
+                for (int r = warp; r < rows; r += kDecodeWarps) {
+                    float mj = -INFINITY, lj = 0.0f;
+#pragma unroll 1
+                    for (int k = lane; k < pieces; k += 32) {
+                        const float mk = __ldcg(piece(k) + kRows * D + r);
+                        const float lk = __ldcg(piece(k) + kRows * D + kRows + r);
+                        if (k < kHeld) wts[k * kRowsMax + r] = mk;
+                        const float mn = fmaxf(mj, mk);
+                        lj = lj * (mj == mn ? 1.0f : weight(mj, mn)) + lk * (mk == mn ? 1.0f : weight(mk, mn));
+                        mj = mn;
+                    }
+                    float mr = mj;
 #pragma unroll
-                for (int off = 4; off > 0; off >>= 1) {
-                    const float mo = __shfl_xor_sync(0xffffffffu, mj, off), lo = __shfl_xor_sync(0xffffffffu, lj, off);
-                    const float mn = fmaxf(mj, mo);
-                    lj = mn == -INFINITY ? lj + lo : lj * ptx::ex2(mj - mn) + lo * ptx::ex2(mo - mn);
-                    mj = mn;
+                    for (int off = 16; off > 0; off >>= 1) mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, off));
+                    lj *= mj == mr ? 1.0f : weight(mj, mr);
+#pragma unroll
+                    for (int off = 16; off > 0; off >>= 1) lj += __shfl_xor_sync(0xffffffffu, lj, off);
+#pragma unroll 1
+                    for (int k = lane; k < min(pieces, kHeld); k += 32)
+                        wts[k * kRowsMax + r] = weight(wts[k * kRowsMax + r], mr);
+                    if (lane == 0) {
+                        stat_m[r] = mr;
+                        stat_l[r] = lj;
+                        write_lse(r, mr, lj);
+                    }
                 }
-                for (int k = threadIdx.x & 7; k < min(pieces, kHeld); k += 8) {
-                    const float mk = wts[k * kRowsMax + row];
-                    wts[k * kRowsMax + row] = mk == -INFINITY ? 0.0f : ptx::ex2(mk - mj);
-                }
-                if ((threadIdx.x & 7) == 0) {
-                    stat_m[row] = mj;
-                    stat_l[row] = lj;
-                }
-                if (row_ok && (threadIdx.x & 7) == 0) write_lse(row, mj, lj);
                 __syncthreads();
-                constexpr int kUnitsMax = kRowsMax * (D / 4) / kDecodeThreads;  // per thread
+                // O in float4 units of the rows, two to a thread; with few rows the pieces are spread over
+                // groups of threads too
                 const int units = rows * (D / 4);
-                const int groups = units >= kDecodeThreads ? 1 : kDecodeThreads / units;
+                const int groups = max(1, kDecodeThreads / units);
                 const int grp = static_cast<int>(threadIdx.x) / units;
-                const int u0 = groups > 1 ? static_cast<int>(threadIdx.x) - grp * units : static_cast<int>(threadIdx.x);
-                float4 x[kUnitsMax];
+                const int u_first = groups > 1 ? static_cast<int>(threadIdx.x) - grp * units : static_cast<int>(threadIdx.x);
+#pragma unroll 1
+                for (int u0 = u_first; u0 < units; u0 += 2 * kDecodeThreads) {
+                    const int u1 = min(u0 + kDecodeThreads, units - 1);
+                    const bool two = u0 + kDecodeThreads < units;
+                    float4 x0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), x1 = x0;
+                    if (groups == 1 || grp < groups) {
+#pragma unroll 1
+                        for (int k0 = groups > 1 ? grp : 0; k0 < pieces; k0 += kJoin * groups) {
+                            float4 y0[kJoin], y1[kJoin];
 #pragma unroll
-                for (int i = 0; i < kUnitsMax; ++i) x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (grp < groups || groups == 1) {
-#pragma unroll 8
-                    for (int k = groups > 1 ? grp : 0; k < pieces; k += groups) {
-                        const float4* pk = reinterpret_cast<const float4*>(piece(k));
+                            for (int i = 0; i < kJoin; ++i) {
+                                const float4* pk = reinterpret_cast<const float4*>(piece(min(k0 + i * groups, pieces - 1)));
+                                y0[i] = __ldcg(pk + u0);
+                                y1[i] = y0[i];
+                                if (two) y1[i] = __ldcg(pk + u1);
+                            }
 #pragma unroll
-                        for (int i = 0; i < kUnitsMax; ++i) {
-                            const int u = u0 + i * kDecodeThreads;
-                            if (u < units) {
-                                const float4 y = __ldcg(pk + u);
-                                const int r = u / (D / 4);
-                                float w;
-                                if (k < kHeld) {
-                                    w = wts[k * kRowsMax + r];
-                                } else {  // one item over most of the GPU
-                                    const float mk = __ldcg(piece(k) + kRowsMax * D + r);
-                                    w = mk == -INFINITY ? 0.0f : ptx::ex2(mk - stat_m[r]);
+                            for (int i = 0; i < kJoin; ++i) {
+                                const int k = k0 + i * groups;
+                                float w0 = 0.0f, w1 = 0.0f;
+                                if (k < pieces && pieces <= kHeld) {
+                                    w0 = wts[k * kRowsMax + u0 / (D / 4)];
+                                    w1 = wts[k * kRowsMax + u1 / (D / 4)];
+                                } else if (k < pieces) {  // one item over most of the GPU
+                                    w0 = weight(__ldcg(piece(k) + kRows * D + u0 / (D / 4)), stat_m[u0 / (D / 4)]);
+                                    w1 = weight(__ldcg(piece(k) + kRows * D + u1 / (D / 4)), stat_m[u1 / (D / 4)]);
                                 }
-                                x[i].x += w * y.x;
-                                x[i].y += w * y.y;
-                                x[i].z += w * y.z;
-                                x[i].w += w * y.w;
+                                x0.x += w0 * y0[i].x;
+                                x0.y += w0 * y0[i].y;
+                                x0.z += w0 * y0[i].z;
+                                x0.w += w0 * y0[i].w;
+                                x1.x += w1 * y1[i].x;
+                                x1.y += w1 * y1[i].y;
+                                x1.z += w1 * y1[i].z;
+                                x1.w += w1 * y1[i].w;
                             }
                         }
                     }
-                }
-                if (groups > 1) {
-                    __syncthreads();  // the weights have been read
-                    float4* sums = reinterpret_cast<float4*>(merge);
-                    if (grp < groups) sums[grp * units + u0] = x[0];
-                    __syncthreads();
-                    if (grp == 0) {
-                        for (int k = 1; k < groups; ++k) {
+                    if (groups > 1) {
+                        __syncthreads();  // the weights have been read
+                        float4* sums = reinterpret_cast<float4*>(merge);
+                        if (grp < groups) sums[threadIdx.x] = x0;
+                        __syncthreads();
+#pragma unroll 1
+                        for (int k = 1; k < groups && grp == 0; ++k) {
                             const float4 y = sums[k * units + u0];
-                            x[0].x += y.x;
-                            x[0].y += y.y;
-                            x[0].z += y.z;
-                            x[0].w += y.w;
+                            x0.x += y.x;
+                            x0.y += y.y;
+                            x0.z += y.z;
+                            x0.w += y.w;
                         }
+                        if (grp != 0) break;
                     }
+                    write_out(u0 / (D / 4), (u0 % (D / 4)) * 4, x0, stat_l[u0 / (D / 4)]);
+                    if (two) write_out(u1 / (D / 4), (u1 % (D / 4)) * 4, x1, stat_l[u1 / (D / 4)]);
                 }
-#pragma unroll
-                for (int i = 0; i < kUnitsMax; ++i) {
-                    const int u = u0 + i * kDecodeThreads;
-                    if (u < units && (groups == 1 || grp == 0))
-                        write_out(u / (D / 4), (u % (D / 4)) * 4, x[i], stat_l[u / (D / 4)]);
-                }
-                __syncthreads();
             }
+            __syncthreads();  // before the next piece writes what was read here
         }
         item0 += cur.n;
         if (!cur.next(a)) break;
@@ -910,39 +1010,56 @@ size_t decode_workspace_bytes(int32_t head_dim) {
 
 namespace {
 
-template <int D, bool kE4M3>
-cudaError_t launch_decode(const DecodeArgs& a, unsigned grid, cudaStream_t stream) {
-    constexpr int smem = DecodeCfg<D, kE4M3>::kSmemBytes;
+template <int D, bool kE4M3, int R>
+cudaError_t launch_decode(DecodeArgs& a, cudaStream_t stream, const char** err) {
+    using Cfg = DecodeCfg<D, kE4M3, R>;
+    a.row_tiles = (a.group + Cfg::kRows - 1) / Cfg::kRows;
+    a.items_per_seq = a.c.heads_kv * a.row_tiles;
+    a.fd_items = make_fastdiv(static_cast<uint32_t>(a.items_per_seq));
+    // no more CTAs than the page table's room could give work to, but one for every piece of few items
+    const int64_t room = static_cast<int64_t>(a.c.max_pages) * a.c.page_size;
+    const int64_t keys = a.window > 0 ? std::min<int64_t>(room, static_cast<int64_t>(a.window) + a.sinks) : room;
+    const int64_t items = static_cast<int64_t>(a.items_per_seq) * a.batch;
+    const int64_t slices = (keys + Cfg::kSlice - 1) / Cfg::kSlice;
+    if (slices * items > 0x7fffffffLL) {  // the kernel counts them in 32 bits
+        *err = "batch x kv-heads x the page table's room is beyond the kernel's 32 bits";
+        return cudaErrorNotSupported;
+    }
+    const int64_t worth = std::max((slices + kMinSlices - 1) / kMinSlices, static_cast<int64_t>(kFewItems)) * items;
+    const int64_t most = std::min<int64_t>(Cfg::kCtas * 148, static_cast<int64_t>(Cfg::kCtas) * a.sm_count);
     const cudaError_t e =
-        cudaFuncSetAttribute(paged_decode_kernel<D, kE4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaFuncSetAttribute(paged_decode_kernel<D, kE4M3, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
     if (e != cudaSuccess) return e;
-    paged_decode_kernel<D, kE4M3><<<grid, kDecodeThreads, smem, stream>>>(a);
+    const unsigned grid = static_cast<unsigned>(std::min(most, worth));
+    paged_decode_kernel<D, kE4M3, R><<<grid, kDecodeThreads, Cfg::kSmemBytes, stream>>>(a);
     return cudaGetLastError();
+}
+
+template <int D, bool kE4M3>
+cudaError_t launch_decode(DecodeArgs& a, cudaStream_t stream, const char** err) {
+    return a.group <= 8 ? launch_decode<D, kE4M3, 1>(a, stream, err) : launch_decode<D, kE4M3, 2>(a, stream, err);
 }
 
 }  // namespace
 
 int launch_paged_decode(DecodeArgs& a, int32_t head_dim, int32_t kv_dtype, cudaStream_t stream, const char** err) {
     static_assert(kDecodeCounterBytes >= kDecodeMaxCtas * sizeof(unsigned int), "a counter per CTA");
-    a.row_tiles = (a.group + kRowsMax - 1) / kRowsMax;
-    a.items_per_seq = a.c.heads_kv * a.row_tiles;
-    // no more CTAs than the page table's room could give work to
-    const int64_t room = static_cast<int64_t>(a.c.max_pages) * a.c.page_size;
-    int64_t keys = room;
-    if (a.window > 0 && static_cast<int64_t>(a.window) + a.sinks < room) keys = static_cast<int64_t>(a.window) + a.sinks;
-    const int64_t slices = (keys + kSlice - 1) / kSlice * a.items_per_seq * a.batch;
-    // and as many as give every piece of few items one of its own
-    const int64_t worth =
-        std::max((slices + kMinSlices - 1) / kMinSlices, static_cast<int64_t>(kFewItems) * a.items_per_seq * a.batch);
-    const int64_t most = std::min<int64_t>(kDecodeMaxCtas, 2 * static_cast<int64_t>(a.sm_count));
-    const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min(most, worth)));
+    a.k16_page = static_cast<uint32_t>(a.c.k_page / 16);
+    a.k16_head = static_cast<uint32_t>(a.c.k_head / 16);
+    a.k16_slot = static_cast<uint32_t>(a.c.k_slot / 16);
+    a.v16_page = static_cast<uint32_t>(a.c.v_page / 16);
+    a.v16_head = static_cast<uint32_t>(a.c.v_head / 16);
+    a.v16_slot = static_cast<uint32_t>(a.c.v_slot / 16);
+    *err = nullptr;
     cudaError_t e;
     if (kv_dtype == ODF_DTYPE_E4M3)
-        e = head_dim == 64 ? launch_decode<64, true>(a, grid, stream) : launch_decode<128, true>(a, grid, stream);
+        e = head_dim == 64 ? launch_decode<64, true>(a, stream, err) : launch_decode<128, true>(a, stream, err);
     else
-        e = head_dim == 64 ? launch_decode<64, false>(a, grid, stream) : launch_decode<128, false>(a, grid, stream);
-    if (e != cudaSuccess) *err = cudaGetErrorString(e);
-    return e == cudaSuccess ? ODF_OK : ODF_ERR_CUDA;
+        e = head_dim == 64 ? launch_decode<64, false>(a, stream, err) : launch_decode<128, false>(a, stream, err);
+    if (e == cudaSuccess) return ODF_OK;
+    if (*err != nullptr) return ODF_ERR_UNSUPPORTED;
+    *err = cudaGetErrorString(e);
+    return ODF_ERR_CUDA;
 }
 
 int launch_paged_append(AppendArgs& a, int32_t head_dim, int32_t kv_dtype, cudaStream_t stream, const char** err) {
