@@ -1919,6 +1919,7 @@ int setup_device_locked(int device, DeviceState& st, const char** err) {
     if (e == cudaSuccess) e = set_kernel_attrs<128, kModWindow | 1>(&regs_ok);
     if (e == cudaSuccess) e = set_kernel_attrs<128, kModWindow | 2>(&regs_ok);
     if (e == cudaSuccess) e = set_kernel_attrs<128, kModWindow | 3>(&regs_ok);
+    if (e == cudaSuccess) e = set_paged_kernel_attrs();
     if (e == cudaSuccess && !regs_ok) {
         st.status_code = ODF_ERR_UNSUPPORTED;
         *err = "flash kernel built with an unexpected register count (the warp register split needs 168)";

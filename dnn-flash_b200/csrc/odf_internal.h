@@ -169,6 +169,9 @@ void* current_context();
 // Device address of the status word bounded waits write to (current device).
 int* device_status_ptr(int device);
 
+// Shared-memory limits of the paged-cache kernels, set with the forward kernels' in ensure_device_ready.
+cudaError_t set_paged_kernel_attrs();
+
 // Its number of SMs (after ensure_device_ready).
 int device_sm_count(int device);
 

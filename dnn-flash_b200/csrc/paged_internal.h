@@ -55,6 +55,7 @@ struct AppendArgs {
     const int32_t* starts;
     const int32_t* counts;
     int32_t batch, tokens;
+    FastDiv fd_tokens, fd_heads;
 };
 
 // Pages are copied as runs of consecutive bytes: a page is heads x slots rows of head_dim

@@ -48,20 +48,6 @@ __device__ __forceinline__ Visible visible_keys(const DecodeArgs& a, int len) {
     return r;
 }
 
-// Byte offsets of a token's K and V rows of head hk, or -1 with a page id out of range.
-__device__ __forceinline__ bool row_offsets(const PagedView& c, const int32_t* table, int j, int hk, int64_t* k, int64_t* v) {
-    const int at = static_cast<int>(fast_div(static_cast<uint32_t>(j), c.fd_page));
-    const int slot = j - at * c.page_size;
-    const int page = __ldg(table + at);
-    if (page < 0 || page >= c.num_pages) {
-        bad_page(c);
-        return false;
-    }
-    *k = page * c.k_page + hk * c.k_head + slot * c.k_slot;
-    *v = page * c.v_page + hk * c.v_head + slot * c.v_slot;
-    return true;
-}
-
 // ------------------------------------------------------------------------------ decode attention
 //
 // What bounds it is the cache: every visible key and value is read once (2 d e bytes a key and
@@ -910,80 +896,163 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
     cp_async_wait<0>();
 }
 
-// A thread per 16 bytes of new row: K, then V.
-__device__ __forceinline__ uint32_t quantise4(const float* x, float scale) {
-    uint32_t r = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        r |= static_cast<uint32_t>(__nv_cvt_float_to_fp8(__fdiv_rn(x[i], scale), __NV_SATFINITE, __NV_E4M3)) << (8 * i);
-    return r;
+// ------------------------------------------------------------------------------ append
+//
+// A copy with a gather of page ids: each new row is read once and written once.  Threads take 16 bytes of a K row
+// and the same of the V row; a block takes kAppendRows rows of (sequence, kv-head, token), the token
+// fastest, which is the order of both sides, and issues all of its loads before its first store.
+constexpr int kAppendThreads = 256;
+constexpr int kAppendUnroll = 4;  // rows of a thread, where that still makes a block for every SM
+
+// A scale as the append kernel divides by it: two factors whose products with a value lie on either side of
+// the fp32 quotient (and are the quotient for a power of two).
+struct Divisor {
+    float scale, lo, hi;
+    bool bracket;  // the reciprocal is a normal number
+    __device__ __forceinline__ explicit Divisor(float s) : scale(s) {
+        const uint32_t u = __float_as_uint(s);
+        const uint32_t e = u >> 23;  // positive scales only (a sign makes e large)
+        bracket = e > 7 && e < 247;
+        const float inv = 1.0f / s;
+        const bool exact = (u & 0x7fffffu) == 0;
+        lo = exact ? inv : inv * (1.0f - 0x1p-21f);
+        hi = exact ? inv : inv * (1.0f + 0x1p-21f);
+    }
+};
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
+           (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16);
 }
 
-template <int D>
-__global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ AppendArgs a, bool e4m3) {
-    constexpr int kVecs = D / 8;
-    const int64_t total = static_cast<int64_t>(a.batch) * a.tokens * a.c.heads_kv * kVecs;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int c = static_cast<int>(i % kVecs);
-        int64_t r = i / kVecs;
-        const int t = static_cast<int>(r % a.tokens);
-        r /= a.tokens;
-        const int hk = static_cast<int>(r % a.c.heads_kv);
-        const int b = static_cast<int>(r / a.c.heads_kv);
-        if (a.counts && t >= __ldg(a.counts + b)) continue;
-        const int64_t pos = static_cast<int64_t>(__ldg(a.starts + b)) + t;
+// Eight bf16 values over a scale, to nearest e4m3 (ties to even), saturated; NaN stays.  Rounding is
+// monotonic, so where the two products round to one e4m3 value the quotient between them does too; where
+// they do not (a quotient within 2^-21 of the middle of two values, about one in 10^5), it is divided.
+// On 100 MB of new rows that takes 42 us, dividing all of them 53 (their bytes: 23 at the copy rate).
+__device__ __forceinline__ uint2 quantise8(uint4 w, const Divisor& d) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(i & 1 ? u[i >> 1] & 0xFFFF0000u : u[i >> 1] << 16);
+    uint2 lo, hi;
+    lo.x = e4m3x4(x[0] * d.lo, x[1] * d.lo, x[2] * d.lo, x[3] * d.lo);
+    hi.x = e4m3x4(x[0] * d.hi, x[1] * d.hi, x[2] * d.hi, x[3] * d.hi);
+    lo.y = e4m3x4(x[4] * d.lo, x[5] * d.lo, x[6] * d.lo, x[7] * d.lo);
+    hi.y = e4m3x4(x[4] * d.hi, x[5] * d.hi, x[6] * d.hi, x[7] * d.hi);
+    if (!d.bracket || lo.x != hi.x || lo.y != hi.y) {
+        lo.x = e4m3x4(x[0] / d.scale, x[1] / d.scale, x[2] / d.scale, x[3] / d.scale);
+        lo.y = e4m3x4(x[4] / d.scale, x[5] / d.scale, x[6] / d.scale, x[7] / d.scale);
+    }
+    return lo;
+}
+
+template <int D, bool kE4M3, int kUnroll>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+    constexpr int kVecs = D / 8;                        // threads of a row
+    constexpr int kRowsPer = kAppendThreads / kVecs;    // rows of a block at a time
+    const int c = threadIdx.x % kVecs;
+    const uint32_t rows = static_cast<uint32_t>(a.batch) * a.tokens * a.c.heads_kv;
+    const uint32_t row0 = blockIdx.x * (kRowsPer * kUnroll) + threadIdx.x / kVecs;
+    // three steps, each with the loads of all rows side by side: starts and counts, then page ids and
+    // the new rows, then the stores
+    int b[kUnroll], h[kUnroll], t[kUnroll], start[kUnroll], count[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+        const uint32_t row = row0 + i * kRowsPer;
+        const uint32_t bh = fast_div(min(row, rows - 1), a.fd_tokens);
+        t[i] = static_cast<int>(min(row, rows - 1) - bh * a.fd_tokens.d);
+        b[i] = static_cast<int>(fast_div(bh, a.fd_heads));
+        h[i] = static_cast<int>(bh) - b[i] * a.c.heads_kv;
+        start[i] = __ldg(a.starts + b[i]);
+        count[i] = a.counts ? __ldg(a.counts + b[i]) : a.tokens;
+        if (row >= rows) count[i] = 0;
+    }
+    int page[kUnroll], slot[kUnroll];
+    uint4 kx[kUnroll], vx[kUnroll];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+        bool ok = t[i] < count[i];
+        const int64_t pos = static_cast<int64_t>(start[i]) + t[i];
         if (pos < 0 || pos >= static_cast<int64_t>(a.c.max_pages) * a.c.page_size) {
-            bad_page(a.c);
+            bad |= ok;
+            ok = false;
+        }
+        const int at = static_cast<int>(fast_div(static_cast<uint32_t>(pos), a.c.fd_page));
+        slot[i] = ok ? static_cast<int>(pos) - at * a.c.page_size : -1;
+        page[i] = ok ? __ldg(a.c.table + b[i] * a.c.table_stride + at) : 0;
+        const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.k) + b[i] * a.k_b + h[i] * a.k_h + t[i] * a.k_t;
+        const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v) + b[i] * a.v_b + h[i] * a.v_h + t[i] * a.v_t;
+        if (ok) kx[i] = __ldg(reinterpret_cast<const uint4*>(k) + c);
+        if (ok) vx[i] = __ldg(reinterpret_cast<const uint4*>(v) + c);
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+        if (slot[i] < 0) continue;
+        if (page[i] < 0 || page[i] >= a.c.num_pages) {
+            bad = true;
             continue;
         }
-        int64_t ko, vo;
-        if (!row_offsets(a.c, a.c.table + b * a.c.table_stride, static_cast<int>(pos), hk, &ko, &vo)) continue;
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(which ? a.v : a.k) +
-                                       (which ? b * a.v_b + hk * a.v_h + t * a.v_t : b * a.k_b + hk * a.k_h + t * a.k_t) + c * 8;
-            uint8_t* dst = which ? a.c.v + vo : a.c.k + ko;
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(src));
-            if (!e4m3) {
-                reinterpret_cast<uint4*>(dst)[c] = w;
-            } else {
-                const float* sp = which ? a.c.v_scale : a.c.k_scale;
-                const float scale = sp ? __ldg(sp + hk) : 1.0f;
-                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[2 * e] = __uint_as_float(u[e] << 16);
-                    x[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
-                }
-                reinterpret_cast<uint2*>(dst)[c] = make_uint2(quantise4(x, scale), quantise4(x + 4, scale));
-            }
+        uint8_t* k = a.c.k + page[i] * a.c.k_page + h[i] * a.c.k_head + slot[i] * a.c.k_slot;
+        uint8_t* v = a.c.v + page[i] * a.c.v_page + h[i] * a.c.v_head + slot[i] * a.c.v_slot;
+        if constexpr (kE4M3) {
+            const float ks = a.c.k_scale ? __ldg(a.c.k_scale + h[i]) : 1.0f;
+            const float vs = a.c.v_scale ? __ldg(a.c.v_scale + h[i]) : 1.0f;
+            reinterpret_cast<uint2*>(k)[c] = quantise8(kx[i], Divisor(ks));
+            reinterpret_cast<uint2*>(v)[c] = quantise8(vx[i], Divisor(vs));
+        } else {
+            reinterpret_cast<uint4*>(k)[c] = kx[i];
+            reinterpret_cast<uint4*>(v)[c] = vx[i];
         }
     }
+    if (bad) bad_page(a.c);
 }
 
-// Pairs travel in the launch's parameters.
+// ------------------------------------------------------------------------------ page copy
+//
+// Pairs travel in the launch's parameters.  A block copies kCopyBytes of a page's K or V in one layer, all of
+// its loads before its first store.
+constexpr int kCopyThreads = 256;
+constexpr int kCopyUnroll = 8;
+constexpr int64_t kCopyBytes = kCopyThreads * kCopyUnroll * 16;
+constexpr int kPairsFew = 16, kPairsMany = 400;  // pairs of a launch
+
 template <int N>
 struct PairList {
     int32_t id[2 * N];
 };
 
 template <int N>
-__global__ void __launch_bounds__(256) page_copy_kernel(const __grid_constant__ CopyArgs a, const __grid_constant__ PairList<N> list) {
+__global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const __grid_constant__ CopyArgs a,
+                                                                 const __grid_constant__ PairList<N> list) {
     const int which = blockIdx.z & 1;
     const int layer = blockIdx.z >> 1;
-    const int pair = blockIdx.x;
-    const int64_t src = list.id[2 * pair] * a.page[which] + layer * a.layer[which];
-    const int64_t dst = list.id[2 * pair + 1] * a.page[which] + layer * a.layer[which];
+    const int pair = blockIdx.y;
+    uint8_t* base = a.base[which] + layer * a.layer[which];
+    const uint8_t* src = base + list.id[2 * pair] * a.page[which];
+    uint8_t* dst = base + list.id[2 * pair + 1] * a.page[which];
     const int64_t vecs = a.run_bytes[which] / 16;
     const int64_t total = vecs * a.inner[which] * a.outer[which];
-    for (int64_t i = static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.y) * blockDim.x) {
-        const int64_t run = i / vecs;
-        const int64_t o = run / a.inner[which];
-        const int64_t off = o * a.outer_stride[which] + (run - o * a.inner[which]) * a.inner_stride[which] + (i - run * vecs) * 16;
-        *reinterpret_cast<uint4*>(a.base[which] + dst + off) = *reinterpret_cast<const uint4*>(a.base[which] + src + off);
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kCopyThreads * kCopyUnroll) + threadIdx.x;
+    if (total == vecs) {  // the page is one run of bytes
+        uint4 x[kCopyUnroll];
+#pragma unroll
+        for (int i = 0; i < kCopyUnroll; ++i)
+            if (first + i * kCopyThreads < total) x[i] = __ldcs(reinterpret_cast<const uint4*>(src) + first + i * kCopyThreads);
+#pragma unroll
+        for (int i = 0; i < kCopyUnroll; ++i)
+            if (first + i * kCopyThreads < total) __stcs(reinterpret_cast<uint4*>(dst) + first + i * kCopyThreads, x[i]);
+        return;
+    }
+#pragma unroll 4
+    for (int i = 0; i < kCopyUnroll; ++i) {
+        const int64_t at = first + i * kCopyThreads;
+        if (at < total) {
+            const int64_t run = at / vecs;
+            const int64_t o = run / a.inner[which];
+            const int64_t off = o * a.outer_stride[which] + (run - o * a.inner[which]) * a.inner_stride[which] + (at - run * vecs) * 16;
+            *reinterpret_cast<uint4*>(dst + off) = __ldg(reinterpret_cast<const uint4*>(src + off));
+        }
     }
 }
 
@@ -991,13 +1060,18 @@ template <int N>
 cudaError_t launch_copy(const CopyArgs& a, int64_t first, int64_t count, cudaStream_t stream) {
     PairList<N> list;
     for (int64_t i = 0; i < 2 * count; ++i) list.id[i] = a.pairs[2 * first + i];
-    for (int l = 0; l < a.layers; l += 32767) {
+    int64_t bytes = 0;
+    for (int w = 0; w < 2; ++w) bytes = std::max(bytes, a.run_bytes[w] * a.inner[w] * a.outer[w]);
+    const int64_t blocks = (bytes + kCopyBytes - 1) / kCopyBytes;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    constexpr int kLayers = 32767;  // of a launch
+    for (int l = 0; l < a.layers; l += kLayers) {
         CopyArgs x = a;
         x.pairs = nullptr;
-        x.layers = a.layers - l < 32767 ? a.layers - l : 32767;
+        x.layers = std::min(a.layers - l, kLayers);
         for (int w = 0; w < 2; ++w) x.base[w] += l * x.layer[w];
-        const dim3 grid(static_cast<unsigned>(count), 4, 2 * x.layers);
-        page_copy_kernel<N><<<grid, 256, 0, stream>>>(x, list);
+        const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(count), 2 * x.layers);
+        page_copy_kernel<N><<<grid, kCopyThreads, 0, stream>>>(x, list);
     }
     return cudaGetLastError();
 }
@@ -1027,9 +1101,6 @@ cudaError_t launch_decode(DecodeArgs& a, cudaStream_t stream, const char** err) 
     }
     const int64_t worth = std::max((slices + kMinSlices - 1) / kMinSlices, static_cast<int64_t>(kFewItems)) * items;
     const int64_t most = std::min<int64_t>(Cfg::kCtas * 148, static_cast<int64_t>(Cfg::kCtas) * a.sm_count);
-    const cudaError_t e =
-        cudaFuncSetAttribute(paged_decode_kernel<D, kE4M3, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
-    if (e != cudaSuccess) return e;
     const unsigned grid = static_cast<unsigned>(std::min(most, worth));
     paged_decode_kernel<D, kE4M3, R><<<grid, kDecodeThreads, Cfg::kSmemBytes, stream>>>(a);
     return cudaGetLastError();
@@ -1041,6 +1112,21 @@ cudaError_t launch_decode(DecodeArgs& a, cudaStream_t stream, const char** err) 
 }
 
 }  // namespace
+
+cudaError_t set_paged_kernel_attrs() {
+    auto set = [](auto kernel, int bytes) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    };
+    cudaError_t e = set(paged_decode_kernel<64, false, 1>, DecodeCfg<64, false, 1>::kSmemBytes);
+    if (e == cudaSuccess) e = set(paged_decode_kernel<64, false, 2>, DecodeCfg<64, false, 2>::kSmemBytes);
+    if (e == cudaSuccess) e = set(paged_decode_kernel<128, false, 1>, DecodeCfg<128, false, 1>::kSmemBytes);
+    if (e == cudaSuccess) e = set(paged_decode_kernel<128, false, 2>, DecodeCfg<128, false, 2>::kSmemBytes);
+    if (e == cudaSuccess) e = set(paged_decode_kernel<64, true, 1>, DecodeCfg<64, true, 1>::kSmemBytes);
+    if (e == cudaSuccess) e = set(paged_decode_kernel<64, true, 2>, DecodeCfg<64, true, 2>::kSmemBytes);
+    if (e == cudaSuccess) e = set(paged_decode_kernel<128, true, 1>, DecodeCfg<128, true, 1>::kSmemBytes);
+    if (e == cudaSuccess) e = set(paged_decode_kernel<128, true, 2>, DecodeCfg<128, true, 2>::kSmemBytes);
+    return e;
+}
 
 int launch_paged_decode(DecodeArgs& a, int32_t head_dim, int32_t kv_dtype, cudaStream_t stream, const char** err) {
     static_assert(kDecodeCounterBytes >= kDecodeMaxCtas * sizeof(unsigned int), "a counter per CTA");
@@ -1062,15 +1148,41 @@ int launch_paged_decode(DecodeArgs& a, int32_t head_dim, int32_t kv_dtype, cudaS
     return ODF_ERR_CUDA;
 }
 
+namespace {
+
+template <int D, bool kE4M3>
+void launch_append(const AppendArgs& a, int64_t rows, cudaStream_t stream) {
+    constexpr int64_t kRowsPer = kAppendThreads / (D / 8);
+    const int64_t wide = (rows + kRowsPer * kAppendUnroll - 1) / (kRowsPer * kAppendUnroll);
+    if (wide >= 148)
+        paged_append_kernel<D, kE4M3, kAppendUnroll><<<static_cast<unsigned>(wide), kAppendThreads, 0, stream>>>(a);
+    else
+        paged_append_kernel<D, kE4M3, 1>
+            <<<static_cast<unsigned>((rows + kRowsPer - 1) / kRowsPer), kAppendThreads, 0, stream>>>(a);
+}
+
+}  // namespace
+
 int launch_paged_append(AppendArgs& a, int32_t head_dim, int32_t kv_dtype, cudaStream_t stream, const char** err) {
     const bool e4m3 = kv_dtype == ODF_DTYPE_E4M3;
-    const int64_t total = static_cast<int64_t>(a.batch) * a.tokens * a.c.heads_kv * (head_dim / 8);
-    const int64_t blocks = (total + 255) / 256;
-    const unsigned grid = static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16);
-    if (head_dim == 64)
-        paged_append_kernel<64><<<grid, 256, 0, stream>>>(a, e4m3);
-    else
-        paged_append_kernel<128><<<grid, 256, 0, stream>>>(a, e4m3);
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens * a.c.heads_kv;
+    if (rows > 0x7fffffffLL) {
+        *err = "batch x kv-heads x tokens is beyond the kernel's 32 bits";
+        return ODF_ERR_UNSUPPORTED;
+    }
+    a.fd_tokens = make_fastdiv(static_cast<uint32_t>(a.tokens));
+    a.fd_heads = make_fastdiv(static_cast<uint32_t>(a.c.heads_kv));
+    if (head_dim == 64) {
+        if (e4m3)
+            launch_append<64, true>(a, rows, stream);
+        else
+            launch_append<64, false>(a, rows, stream);
+    } else {
+        if (e4m3)
+            launch_append<128, true>(a, rows, stream);
+        else
+            launch_append<128, false>(a, rows, stream);
+    }
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) *err = cudaGetErrorString(e);
     return e == cudaSuccess ? ODF_OK : ODF_ERR_CUDA;
@@ -1079,9 +1191,8 @@ int launch_paged_append(AppendArgs& a, int32_t head_dim, int32_t kv_dtype, cudaS
 int launch_page_copy(const CopyArgs& a, cudaStream_t stream, const char** err) {
     cudaError_t e = cudaSuccess;
     for (int64_t first = 0; first < a.n_pairs && e == cudaSuccess;) {
-        const int64_t left = a.n_pairs - first;
-        const int64_t count = left < 400 ? left : 400;
-        e = count <= 16 ? launch_copy<16>(a, first, count, stream) : launch_copy<400>(a, first, count, stream);
+        const int64_t count = std::min<int64_t>(a.n_pairs - first, kPairsMany);
+        e = count <= kPairsFew ? launch_copy<kPairsFew>(a, first, count, stream) : launch_copy<kPairsMany>(a, first, count, stream);
         first += count;
     }
     if (e != cudaSuccess) *err = cudaGetErrorString(e);

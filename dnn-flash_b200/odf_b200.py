@@ -312,7 +312,7 @@ def flash_fwd_window(q, k, v, *, window, sinks=0, q_offset=0, scale=None, alibi=
     slopes = _slopes_array(alibi_slopes, Hq) if alibi else None
     where, handle = _launch_on(dev, stream)
     with where:
-        out, lse = _outputs(q, out, lse_out, out_dtype, want_lse, dev)
+        out, lse = _outputs(q, out, lse_out, out_dtype, want_lse)
         p = FwdParams(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
                       ODF_DTYPE_BF16, ODF_DTYPE_BF16 if out.dtype == torch.bfloat16 else ODF_DTYPE_F32, B, Hq, k.shape[1], M,
                       k.shape[2], D, D, _strides(q, "q"), _strides(k, "k"), _strides(v, "v"), _strides(out, "out"),
@@ -406,11 +406,13 @@ _NO_STRIDES2 = (C.c_int64 * 2)()
 
 
 def _strides(t, name):
-    """Element strides of all dimensions but the last, which must be contiguous; all zero = contiguous."""
+    """Element strides of (up to three) dimensions before the last, which must be contiguous; all zero = contiguous."""
     n = t.dim() - 1
     if t.is_contiguous():
-        return _NO_STRIDES3 if n == 3 else _NO_STRIDES2
+        return _NO_STRIDES2 if n == 2 else _NO_STRIDES3
     shape, stride = t.shape, t.stride()
+    if n == 4:  # layers, which have a stride of their own
+        n, shape, stride = 3, shape[1:], stride[1:]
     if stride[n] != 1:
         raise ValueError(f"the innermost (feature) dimension of {name} must be contiguous")
     out, dense = list(stride[:n]), shape[n]
@@ -448,17 +450,18 @@ def _scale_ptr(tensor, name, device, heads):
 
 
 def _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, device, batch, heads=None, head_dim=None):
-    """odf_paged_cache of one layer's pages (PagedCache), checked against the call's other tensors."""
+    """odf_paged_cache of one layer's pages (PagedCache), checked against the call's other tensors.  Without
+    a page table the pages may have a leading dimension of layers (page_copy)."""
     import torch
 
     shape, dtype = k_pages.shape, k_pages.dtype
-    if len(shape) != 4 or v_pages.shape != shape:
+    if v_pages.shape != shape or (len(shape) != 4 and (page_table is not None or len(shape) != 5)):
         raise ValueError("k_pages and v_pages must be rank 4 [pages, heads_kv, page_size, head_dim] of one shape")
     if v_pages.dtype != dtype or dtype not in (torch.bfloat16, torch.float8_e4m3fn):
         raise ValueError(f"a cache holds bfloat16 or float8_e4m3fn, not {dtype} and {v_pages.dtype}")
     _on(k_pages, "k_pages", device)
     _on(v_pages, "v_pages", device)
-    pages, hkv, page_size, dim = shape
+    pages, hkv, page_size, dim = shape if len(shape) == 4 else shape[1:]
     if (heads is not None and heads != hkv) or (head_dim is not None and head_dim != dim):
         raise ValueError("the new tensors and the cache must have the same kv-heads and head_dim")
     table, table_stride, max_pages = None, 0, 0
@@ -528,19 +531,24 @@ def _require_cuda(device):
         raise ValueError(f"tensors must be on a CUDA device, not {device}")
 
 
-def _outputs(q, out, lse_out, out_dtype, want_lse, device):
+def _outputs(q, out, lse_out, out_dtype, want_lse):
     """The given or new outputs of an attention call with q's shape."""
     import torch
 
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or torch.float32, device=device)
+        dtype = out_dtype or torch.float32
+        # the short forms of torch.empty(q.shape, dtype=..., device=...), which costs 2 us more
+        out = torch.empty_like(q) if dtype is q.dtype and q.is_contiguous() else q.new_empty(q.shape, dtype=dtype)
     else:
-        _on(out, "out", device)
-    if out.shape != q.shape or out.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError("out must be float32 or bfloat16 of q's shape")
+        dtype = out.dtype
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+        _on(out, "out", q.device)
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise ValueError("out must be float32 or bfloat16")
     if lse_out is None:
-        return out, torch.empty(q.shape[:-1], dtype=torch.float32, device=device) if want_lse else None
-    _on(lse_out, "lse_out", device)
+        return out, q.new_empty(q.shape[:-1], dtype=torch.float32) if want_lse else None
+    _on(lse_out, "lse_out", q.device)
     if lse_out.shape != q.shape[:-1] or lse_out.dtype != torch.float32 or not lse_out.is_contiguous():
         raise ValueError("lse_out must be contiguous float32 of q's shape without its last dimension")
     return out, lse_out
@@ -589,7 +597,7 @@ def paged_decode(q, k_pages, v_pages, page_table, lens, *, scale=None, window=0,
     slopes = _slopes_array(alibi_slopes, Hq) if alibi else None
     where, handle = _launch_on(dev, stream)
     with where:
-        out, lse = _outputs(q, out, lse_out, out_dtype, want_lse, dev)
+        out, lse = _outputs(q, out, lse_out, out_dtype, want_lse)
         if workspace is None:
             workspace = paged_decode_workspace(B, Hq, cache.heads_kv, D, device=dev)
         else:
@@ -634,10 +642,9 @@ def page_copy(k_pages, v_pages, pairs, *, stream=None):
     """
     import numpy as np
 
-    layered = k_pages.dim() == 5
-    if k_pages.dim() not in (4, 5) or k_pages.shape != v_pages.shape or (layered and k_pages.shape[0] == 0):
+    rank, shape, dev = k_pages.dim(), k_pages.shape, k_pages.device
+    if rank not in (4, 5) or v_pages.shape != shape:
         raise ValueError("k_pages and v_pages must be [pages, Hkv, page_size, D] or [layers, pages, ...] of one shape")
-    dev = k_pages.device
     _require_cuda(dev)
     ids = np.asarray(pairs)
     if ids.size == 0:
@@ -645,15 +652,17 @@ def page_copy(k_pages, v_pages, pairs, *, stream=None):
     if ids.ndim != 2 or ids.shape[1] != 2 or ids.dtype.kind not in "iu":
         raise ValueError("pairs must be integers of shape [n, 2]")
     if ids.dtype != np.int32:
-        if int(ids.min()) < 0 or int(ids.max()) >= k_pages.shape[-4]:  # before they are cut to 32 bits
+        ids = np.ascontiguousarray(ids, dtype=np.int64)
+        if ids.view(np.uint64).max() >= shape[-4]:  # before they are cut to 32 bits; negative ids are large here
             raise ValueError("a page id is outside the cache")
-        ids = ids.astype(np.int32)
-    ids = np.ascontiguousarray(ids)
-    if layered:
-        cache = _cache_params(k_pages[0], v_pages[0], None, None, None, dev, 0)
-        p = PageCopyParams(cache, k_pages.shape[0], k_pages.stride(0), v_pages.stride(0), ids.ctypes.data, len(ids))
-    else:
-        p = PageCopyParams(_cache_params(k_pages, v_pages, None, None, None, dev, 0), 1, 0, 0, ids.ctypes.data, len(ids))
+    ids = np.ascontiguousarray(ids, dtype=np.int32)
+    cache = _cache_params(k_pages, v_pages, None, None, None, dev, 0)
+    layers, k_layer, v_layer = 1, 0, 0
+    if rank == 5:
+        layers, k_layer, v_layer = shape[0], k_pages.stride(0), v_pages.stride(0)
+        if layers == 0:
+            raise ValueError("the cache has no layers")
+    p = PageCopyParams(cache, layers, k_layer, v_layer, ids.ctypes.data, len(ids))
     where, handle = _launch_on(dev, stream)
     with where:
         _check(load_library().odf_page_copy_sm100(C.byref(p), handle))

@@ -256,6 +256,26 @@ def test_append(kv, layout, B, Hkv, T, D, page):
             assert torch.equal(torch.nan_to_num(pages.float(), nan=12345.0), torch.nan_to_num(want.float(), nan=12345.0))
 
 
+def test_append_rounds_every_value_as_the_quotient():
+    """All bf16 values over scales of every kind: the e4m3 value of the fp32 quotient, ties and subnormals included."""
+    x = torch.arange(65536, device="cuda", dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    scales = [1.0, 1 / 64, 0.015625 * 1.5, 0.1, 1 / 3, 7.123e-3, 0.99999994, 1.0000001, 3e-39, 1e38, 2.0 ** -126, 2.0 ** 127,
+              2.0 ** 100, 1.1e-30, 5.0, 1e-45]
+    Hkv, D, page = len(scales), 128, 64
+    tokens = 65536 // D
+    k = x.view(1, 1, tokens, D).expand(1, Hkv, tokens, D).contiguous()
+    s = torch.tensor(scales, device="cuda")
+    table = torch.arange(tokens // page, device="cuda", dtype=torch.int32).view(1, -1)
+    pages = [torch.zeros((tokens // page, Hkv, page, D), device="cuda").to(torch.float8_e4m3fn) for _ in range(2)]
+    odf.paged_append(k, k.flip(1), pages[0], pages[1], table, torch.zeros(1, device="cuda", dtype=torch.int32),
+                     k_scale=s, v_scale=s.flip(0))
+    want = ref.to_e4m3((k[0].float() / s.view(-1, 1, 1)).double())
+    got = pages[0].transpose(0, 1).reshape(Hkv, tokens, D).float()
+    assert torch.equal(torch.nan_to_num(got, nan=999.0), torch.nan_to_num(want.float(), nan=999.0))
+    got = pages[1].transpose(0, 1).reshape(Hkv, tokens, D).float().flip(0)
+    assert torch.equal(torch.nan_to_num(got, nan=999.0), torch.nan_to_num(want.float(), nan=999.0))
+
+
 # ----------------------------------------------------------------------------------------- copy
 @pytest.mark.parametrize("kv", ["bf16", "e4m3"])
 @pytest.mark.parametrize("layout", ["HND", "NHD", "padded"])
