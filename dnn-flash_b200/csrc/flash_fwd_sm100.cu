@@ -144,7 +144,7 @@ struct Config {
     static constexpr uint32_t kOffBar = kOffSlots + kSlots * kTileBytes;
     static constexpr int kNumBars = 2 + 2 * kSlots + 2 + 2 + 2 + 2 + 2 + 2 * kItemQueue + 1;
     static constexpr uint32_t kOffRows = kOffBar + kNumBars * 8 + 16;  // after the barriers, TMEM slot, abort flag
-    static constexpr uint32_t kOffQueue = kOffRows + 8 * 48;             // item queue (int64 x kItemQueue)
+    static constexpr uint32_t kOffQueue = kOffRows + 8 * 64;             // item queue (int64 x kItemQueue)
     // same-shape bias: 2 KB per softmax warp to transpose coalesced row reads (32 rows x 16 keys)
     static constexpr uint32_t kOffBias = (kOffQueue + 8 * kItemQueue + 127) & ~127u;  // float4 stores
     static_assert(kOffBias % 16 == 0 && kOffRows % 8 == 0 && kOffQueue % 8 == 0, "shared-memory alignment");
@@ -177,8 +177,9 @@ struct Bars {
 // warp, written by lane 0) and read where needed, so that no registers stay tied up
 // across the softmax loop.
 struct RowItem {
-    int n_entries;  // KV tiles of the pair (reversed walk: up to and including the diagonal)
-    int pair;
+    int n_entries;  // KV tiles of the pair (reversed walk: up to and including the diagonal; sliding
+                    // window: the first tile that is visible as a whole to the warp's rows)
+    int pair;       // (sliding window: the tile that this query tile leaves out)
     int q0;         // first row of this warp's query tile
     int n_iter;     // list mode: n_entries; dense/causal: the KV tiles this query tile needs (0..n_iter-1)
     int bh, b, h;
@@ -186,8 +187,11 @@ struct RowItem {
     int64_t bias_off;  // same-shape bias: element offset of this (batch, head)'s plane
     int kv0;           // first KV tile of the item's split of the key range
     int split;         // which split (0 without KV splits)
+    int n_full;        // sliding window: how many tiles from n_entries on are visible as a whole,
+    int win_end, win_n;  // the end of this query tile's tiles and the number of the pair's
+    int pad;
 };
-static_assert(sizeof(RowItem) == 48, "RowItem layout");
+static_assert(sizeof(RowItem) == 64, "RowItem layout");
 
 // KV tile j of this query-tile pair: kv index in the low 16 bits, kNeed*/kBitmap* flags above.
 // With KV splits, entry j of an item is KV tile kv0 + j of its split (dense and causal modes).
@@ -216,7 +220,7 @@ struct Item {
     int n_entries;     // KV tiles visited by the pair (entries 0 .. n_entries - 1 of kv_entry)
     bool valid1;       // Q1 has rows
     int split, kv0;    // KV split of the item and its first KV tile (0, 0 without splits)
-    int win_lo, n_sink;  // sliding window: first key of its tiles, and the sink tiles before them
+    int win_lo, n_sink, win_n;  // sliding window: first key of its tiles, the sink tiles before them, all tiles
 };
 
 // Sliding window.  Row qi sits at position p = q_offset + qi and sees the keys j <= p with
@@ -244,12 +248,29 @@ __device__ __forceinline__ WindowSpan window_span(const FwdArgs& a, int q00, int
     return w;
 }
 
-// First key of the pair's tile t, and whether a query tile with rows at positions [p0, pe) needs it.
+// Order of the pair's n tiles: from the first key on, which keeps the tile that only Q1 needs at an item's end
+// and the one that only Q0 needs near its start, where they overlap with the neighbouring items.  ALiBi goes from
+// the diagonal down, so that tiles whose scores no longer count meet a settled max (kFarLog2): 32 heads
+// of 8192 rows, window 1024: 412 -> 345 us.
+template <bool kAlibi>
+__device__ __forceinline__ int window_tile(int j, int n) {
+    return kAlibi ? n - 1 - j : j;
+}
+// First key of the pair's tile t.
 __device__ __forceinline__ int window_tile_start(int t, int lo, int n_sink) {
     return t < n_sink ? t * kTileK : lo + (t - n_sink) * kTileK;
 }
-__device__ __forceinline__ bool window_tile_needed(const FwdArgs& a, int start, bool sink, int p0, int pe) {
-    return start < pe && (sink || start + kTileK > p0 - a.window + 1 || start < a.sinks);
+// The pair's tiles that a query tile with rows at positions [p0, pe) visits: all up to (not including) `end`,
+// but `skip`: the first window tile, which lies before the window of every row of Q1 (unless the run starts at
+// key 0, where the sinks may be).
+struct WindowVisit {
+    int end, skip;
+};
+__device__ __forceinline__ WindowVisit window_visit(const FwdArgs& a, int lo, int n_sink, int p0, int pe) {
+    WindowVisit v;
+    v.end = n_sink + max(0, (min(a.n, pe) - lo + kTileK - 1) / kTileK);
+    v.skip = lo > 0 && p0 - a.window + 1 >= lo + kTileK ? n_sink : -1;
+    return v;
 }
 
 // Items come in blocks of units_per_block (batch, kv-head) units: inside a block, item i is
@@ -257,7 +278,7 @@ __device__ __forceinline__ bool window_tile_needed(const FwdArgs& a, int start, 
 // block (G = q-heads per kv-head).  A block's K/V fits in L2 while its CTAs stream through it.
 // With one block holding every unit this is plain pair-major order over all heads.  With KV
 // splits, the n_splits splits of a pair's key range are consecutive items.
-template <bool kWin>
+template <int MOD>
 __device__ __forceinline__ Item decode_item(const FwdArgs& a, int64_t k) {
     Item I;
     I.split = 0;
@@ -328,11 +349,12 @@ __device__ __forceinline__ Item decode_item(const FwdArgs& a, int64_t k) {
     I.valid1 = I.q01 < a.m;
     I.qend0 = min(a.m, I.q00 + kTileQ);
     I.qend1 = I.valid1 ? min(a.m, I.q01 + kTileQ) : I.qend0;
-    if constexpr (kWin) {
+    if constexpr ((MOD & kModWindow) != 0) {
         const WindowSpan w = window_span(a, I.q00, I.qend1);
         I.win_lo = w.lo;
         I.n_sink = w.n_sink;
-        I.n_entries = w.n_sink + w.n_win;
+        I.win_n = w.n_sink + w.n_win;
+        I.n_entries = I.win_n;
     } else if (a.mode == kModeList) {
         I.n_entries = a.tile_count[I.pair];
     } else if (a.mode == kModeCausal) {
@@ -346,15 +368,15 @@ __device__ __forceinline__ Item decode_item(const FwdArgs& a, int64_t k) {
     return I;
 }
 
-template <bool kWin>
+template <int MOD>
 __device__ __forceinline__ uint32_t kv_entry(const FwdArgs& a, const Item& I, int j) {
-    if constexpr (kWin) {
-        const int t = I.kv0 + j;
-        const int start = window_tile_start(t, I.win_lo, I.n_sink);
-        const bool sink = t < I.n_sink;
+    if constexpr ((MOD & kModWindow) != 0) {
+        const int t = window_tile<(MOD & kModAlibi) != 0>(I.kv0 + j, I.win_n);
+        const WindowVisit v0 = window_visit(a, I.win_lo, I.n_sink, a.q_offset + I.q00, a.q_offset + I.qend0);
+        const WindowVisit v1 = window_visit(a, I.win_lo, I.n_sink, a.q_offset + I.q01, a.q_offset + I.qend1);
         uint32_t e = static_cast<uint32_t>(t);
-        if (window_tile_needed(a, start, sink, a.q_offset + I.q00, a.q_offset + I.qend0)) e |= kNeed0;
-        if (I.valid1 && window_tile_needed(a, start, sink, a.q_offset + I.q01, a.q_offset + I.qend1)) e |= kNeed1;
+        if (t < v0.end && t != v0.skip) e |= kNeed0;
+        if (I.valid1 && t < v1.end && t != v1.skip) e |= kNeed1;
         return e;
     }
     return kv_entry(a, I.pair, j, I.valid1, I.qend0, I.qend1, I.kv0);
@@ -544,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         k = static_item(n_items, it);  // every role computes the same sequence
                     }
                     if (k < 0) break;
-                    const Item I = decode_item<kWin>(args, k);
+                    const Item I = decode_item<MOD>(args, k);
                     ODF_CHECK(I.pair >= 0 && I.pair < args.n_pairs && I.bh >= 0 &&
                                   I.bh < args.batch * args.heads_q && I.hk >= 0 && I.hk < args.heads_kv &&
                                   I.n_entries >= 0 && I.n_entries <= args.n_kt + (kWin ? 1 : 0),
@@ -567,12 +589,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     ++q_loads;
                     for (int j = 0; ok && j < I.n_entries; ++j) {
-                        const int kt = static_cast<int>(kv_entry<kWin>(args, I, j) & 0xFFFFu);
+                        const int kt = static_cast<int>(kv_entry<MOD>(args, I, j) & 0xFFFFu);
                         int row0 = kt * kTileK;  // first key of the tile
                         if constexpr (kWin) row0 = window_tile_start(kt, I.win_lo, I.n_sink);
 #ifdef ODF_CHECKED
                         {
-                            const uint32_t e_chk = kv_entry<kWin>(args, I, j);
+                            const uint32_t e_chk = kv_entry<MOD>(args, I, j);
                             ODF_CHECK((kWin || kt < args.n_kt) && row0 >= 0 && row0 < args.n &&
                                           (e_chk & (kNeed0 | kNeed1)) != 0 && (I.valid1 || !(e_chk & kNeed1)),
                                       1);
@@ -728,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             k = static_item(n_items, it);
                         }
                         if (k < 0) return false;
-                        In = decode_item<kWin>(args, k);
+                        In = decode_item<MOD>(args, k);
                         if (In.n_entries > 0) return true;
                     }
                 };
@@ -736,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 int it = -1;
                 Item I;
                 const bool have = next_nonempty(it, I);
-                uint32_t e = have ? kv_entry<kWin>(args, I, 0) : 0u;
+                uint32_t e = have ? kv_entry<MOD>(args, I, 0) : 0u;
                 if (have) ok = start_item(I, e, 0);
                 for (int j = 0, g = 0; have && ok; ++g) {
                     const int tv = 2 * g + 1;  // V of the current entry
@@ -747,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!last && Cfg::kSepP) {
                         // separate P: the next S MMAs go first (they only wait for the softmax to
                         // have read S), then this tile's P.V MMAs as each P_i arrives
-                        const uint32_t en = kv_entry<kWin>(args, I, j + 1);
+                        const uint32_t en = kv_entry<MOD>(args, I, j + 1);
                         if (!(ok = wait_full(tk))) break;
                         ptx::tc_fence_after();
                         if ((en & kNeed0) && !(ok = issue_s(0, tk % kSlots))) break;
@@ -760,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         e = en;
                         ++j;
                     } else if (!last) {
-                        const uint32_t en = kv_entry<kWin>(args, I, j + 1);
+                        const uint32_t en = kv_entry<MOD>(args, I, j + 1);
                         if ((e & kNeed0) && !(ok = issue_pv(0, tv % kSlots))) break;
                         if (!(ok = wait_full(tk))) break;
                         ptx::tc_fence_after();
@@ -781,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (acc[1]) ptx::tc_commit(&bars.o_done[1]);
                         acc[0] = acc[1] = false;
                         if (!next_nonempty(it, I)) break;
-                        e = kv_entry<kWin>(args, I, 0);
+                        e = kv_entry<MOD>(args, I, 0);
                         j = 0;
                         if (!(ok = start_item(I, e, tk))) break;
                     }
@@ -861,15 +883,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (item < 0) break;
             __syncwarp();  // every lane is done with the previous record
             if (lane == 0) {
-                const Item I = decode_item<kWin>(args, item);
+                const Item I = decode_item<MOD>(args, item);
                 RowItem r;
                 // reversed walk: entry j is KV tile n_entries - 1 - j, counted from the top tile
+                r.n_full = 0;
                 r.n_entries = args.kv_reverse ? min(args.n_kt, (I.qend1 + kTileK - 1) / kTileK) : I.n_entries;
                 r.pair = I.pair;
                 r.q0 = qtile == 0 ? I.q00 : I.q01;
                 const bool valid = qtile == 0 || I.valid1;
-                if (kWin) {
+                if constexpr (kWin) {
+                    const int p0 = args.q_offset + r.q0;
+                    const WindowVisit v =
+                        window_visit(args, I.win_lo, I.n_sink, p0, args.q_offset + min(args.m, r.q0 + kTileQ));
                     r.n_iter = valid ? I.n_entries : 0;
+                    r.pair = v.skip;
+                    r.win_end = v.end;
+                    r.win_n = I.win_n;
+                    // tiles [full, full + n_full) of the window are visible as a whole to this warp's rows
+                    const int wp0 = p0 + (warp & 3) * 32;
+                    const int seen = min(wp0 + 1, args.n) - I.win_lo;  // keys that the first row reaches, from win_lo on
+                    const int first = args.sinks >= args.n ? 0 : max(0, wp0 + 32 - args.window - I.win_lo);
+                    const int full = (first + kTileK - 1) / kTileK;
+                    r.n_entries = I.n_sink + full;
+                    r.n_full = max(0, (seen < 0 ? 0 : seen / kTileK) - full);
                 } else if (args.mode == kModeList) {
                     r.n_iter = I.n_entries;
                 } else if (!valid) {
@@ -914,7 +950,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     e = __ldg(args.tile_list + static_cast<int64_t>(rec->pair) * args.n_kt + j);
                     if (!(e & need_bit)) continue;
                 }
-                const int kt = static_cast<int>(e & 0xFFFFu);
+                int kt = static_cast<int>(e & 0xFFFFu);
                 const int q0 = rec->q0;  // loaded ahead of the wait, which hides its latency
                 int k0 = kt * kTileK;
                 bool sink_tile = false;
@@ -924,16 +960,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (kWin) {
                     const int64_t span = rec->bias_off;
                     const int n_sink = static_cast<int>(span >> 32);
+                    kt = window_tile<(MOD & kModAlibi) != 0>(rec->kv0 + j, rec->win_n);
+                    if (kt == rec->pair || kt >= rec->win_end) continue;
                     sink_tile = kt < n_sink;
                     k0 = window_tile_start(kt, static_cast<int>(span), n_sink);
-                    const int p0 = args.q_offset + q0;
-                    if (!window_tile_needed(args, k0, sink_tile, p0, args.q_offset + min(args.m, q0 + kTileQ))) continue;
-                    const int wp0 = p0 + wq * 32;
-                    const bool in_sinks = k0 + kTileK <= args.sinks;
-                    win_low = !sink_tile && !in_sinks && k0 <= wp0 + 31 - args.window;
-                    win_full = !win_low && k0 + kTileK - 1 <= wp0 && k0 + kTileK <= (sink_tile ? args.sinks : args.n);
-                    win_none = k0 > wp0 + 31 ||
-                               (!sink_tile && k0 >= args.sinks && k0 + kTileK - 1 <= wp0 - args.window);
+                    win_full = static_cast<uint32_t>(kt - rec->n_entries) < static_cast<uint32_t>(rec->n_full);
+                    if (!win_full) {
+                        const int wp0 = args.q_offset + q0 + wq * 32;
+                        win_full = sink_tile && k0 + kTileK <= args.sinks;
+                        win_low = !sink_tile && k0 <= wp0 + 31 - args.window;
+                        win_none = !sink_tile && (k0 > wp0 + 31 || (k0 >= args.sinks && k0 + kTileK - 1 <= wp0 - args.window));
+                    }
                 }
                 // Waits are per thread; the warp re-converges (and agrees) before the
                 // .sync.aligned TMEM accesses that follow.
@@ -970,7 +1007,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // moves only past 2^8, which a sum of at most 2^8 rules out; otherwise S is read
                     // again and the general path below runs (with the same P where the max stays), so
                     // the result is the same as with the max pass first.
-                    const bool interior = kWin ? win_full
+                    // (sliding window: not the first whole tile either, whose max the row has yet to see)
+                    const bool interior = kWin ? win_full && kt != rec->n_entries
                                                : k0 + kTileK <= args.n && !(e & bitmap_bit) &&
                                                      !(args.causal && k0 + kTileK - 1 > q0);
                     if (args.scale_log2 > 0.0f && interior && __all_sync(0xffffffffu, m_run != -INFINITY)) {
@@ -1233,9 +1271,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 float alpha = 1.0f;
+                // Sliding window with the row-sum check: the first tile of a row may hold few visible keys
+                // (sinks, the window's edge), whose max would leave every later sum past the check, so
+                // the max moves at once whenever a tile comes this way (64 heads of 32768 rows, window 4096
+                // and 4 sinks: 5.39 -> 3.83 ms).
+                constexpr float kRaise = kWin && (MOD & kModSkipMax) ? 0.0f : kRescaleLog2;
                 if (m_run == -INFINITY) {
                     m_run = tile_max;  // first valid tile of this row: O holds zeros so far
-                } else if (tile_max > m_run + kRescaleLog2) {
+                } else if (tile_max > m_run + kRaise) {
                     alpha = ptx::ex2(m_run - tile_max);
                     m_run = tile_max;
                 }
