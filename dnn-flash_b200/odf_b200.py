@@ -537,8 +537,8 @@ def _outputs(q, out, lse_out, out_dtype, want_lse):
 
     if out is None:
         dtype = out_dtype or torch.float32
-        # the short forms of torch.empty(q.shape, dtype=..., device=...), which costs 2 us more
-        out = torch.empty_like(q) if dtype is q.dtype and q.is_contiguous() else q.new_empty(q.shape, dtype=dtype)
+        # the short forms of torch.empty(q.shape, dtype=..., device=...), which costs 1 us more
+        out = torch.empty_like(q, dtype=dtype) if q.is_contiguous() else q.new_empty(q.shape, dtype=dtype)
     else:
         dtype = out.dtype
         if out.shape != q.shape:
@@ -547,7 +547,7 @@ def _outputs(q, out, lse_out, out_dtype, want_lse):
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise ValueError("out must be float32 or bfloat16")
     if lse_out is None:
-        return out, q.new_empty(q.shape[:-1], dtype=torch.float32) if want_lse else None
+        return out, q.new_empty(*q.shape[:-1], dtype=torch.float32) if want_lse else None
     _on(lse_out, "lse_out", q.device)
     if lse_out.shape != q.shape[:-1] or lse_out.dtype != torch.float32 or not lse_out.is_contiguous():
         raise ValueError("lse_out must be contiguous float32 of q's shape without its last dimension")
