@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import os
+import struct
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -95,6 +96,16 @@ class PageCopyParams(C.Structure):
     ]
 
 
+# The same structs as one struct.pack call each, in field order (ctypes takes three times as long to
+# build them, as long as a short kernel runs).
+_CACHE_FORMAT = "PPi4q3q3qPPPqq"
+_PACK_DECODE = struct.Struct("@PPPi2q2q2qP" + _CACHE_FORMAT + "fqqiPfPN").pack
+_PACK_APPEND = struct.Struct("@PPqq3q3qPP" + _CACHE_FORMAT).pack
+_PACK_COPY = struct.Struct("@" + _CACHE_FORMAT + "qqqPq").pack
+_PACK_FWD = struct.Struct("@5Pii7q3q3q3q3qfiP4qiPfPNPP4q").pack
+_PACK_WINDOW = struct.Struct("@qqq").pack
+
+
 class OdfError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"odf status {code}: {message}")
@@ -116,18 +127,19 @@ def load_library():
     lib.odf_flash_fwd_host.argtypes = [C.POINTER(FwdParams)]
     lib.odf_fwd_workspace_size.argtypes = [C.POINTER(FwdParams)]
     lib.odf_fwd_workspace_size.restype = C.c_size_t
-    lib.odf_flash_fwd_window_sm100.argtypes = [C.POINTER(FwdParams), C.POINTER(Window), C.c_void_p]
-    lib.odf_fwd_window_workspace_size.argtypes = [C.POINTER(FwdParams), C.POINTER(Window)]
+    # c_void_p takes a packed struct (bytes), byref() of a ctypes one, or None
+    lib.odf_flash_fwd_window_sm100.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.odf_fwd_window_workspace_size.argtypes = [C.c_void_p, C.c_void_p]
     lib.odf_fwd_window_workspace_size.restype = C.c_size_t
     lib.odf_tile_map_sm100.argtypes = [C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_int64,
                                        C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]
     lib.odf_convert_f32_to_bf16.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
     lib.odf_device_status.argtypes = [C.POINTER(C.c_int32), C.c_int32]
-    lib.odf_paged_decode_sm100.argtypes = [C.POINTER(DecodeParams), C.c_void_p]
-    lib.odf_paged_decode_workspace_size.argtypes = [C.POINTER(DecodeParams)]
+    lib.odf_paged_decode_sm100.argtypes = [C.c_void_p, C.c_void_p]
+    lib.odf_paged_decode_workspace_size.argtypes = [C.c_void_p]
     lib.odf_paged_decode_workspace_size.restype = C.c_size_t
-    lib.odf_paged_append_sm100.argtypes = [C.POINTER(AppendParams), C.c_void_p]
-    lib.odf_page_copy_sm100.argtypes = [C.POINTER(PageCopyParams), C.c_void_p]
+    lib.odf_paged_append_sm100.argtypes = [C.c_void_p, C.c_void_p]
+    lib.odf_page_copy_sm100.argtypes = [C.c_void_p, C.c_void_p]
     i64, p64, p32 = C.c_int64, C.POINTER(C.c_int64), C.c_void_p
     lib.odf_page_pool_create.argtypes = [i64, i64, C.POINTER(C.c_void_p)]
     lib.odf_page_pool_destroy.argtypes = [C.c_void_p]
@@ -302,7 +314,8 @@ def flash_fwd_window(q, k, v, *, window, sinks=0, q_offset=0, scale=None, alibi=
     lib = load_library()
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError("q must be [B, Hq, M, D], k and v of one shape [B, Hkv, N, D]")
-    if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+    bf16 = torch.bfloat16
+    if q.dtype is not bf16 or k.dtype is not bf16 or v.dtype is not bf16:
         raise ValueError("q, k and v must be bfloat16")
     B, Hq, M, D = q.shape
     dev = q.device
@@ -313,18 +326,18 @@ def flash_fwd_window(q, k, v, *, window, sinks=0, q_offset=0, scale=None, alibi=
     where, handle = _launch_on(dev, stream)
     with where:
         out, lse = _outputs(q, out, lse_out, out_dtype, want_lse)
-        p = FwdParams(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-                      ODF_DTYPE_BF16, ODF_DTYPE_BF16 if out.dtype == torch.bfloat16 else ODF_DTYPE_F32, B, Hq, k.shape[1], M,
-                      k.shape[2], D, D, _strides(q, "q"), _strides(k, "k"), _strides(v, "v"), _strides(out, "out"),
-                      1.0 / math.sqrt(D) if scale is None else scale, 1, None, 0, 0, 0, 0,
-                      ODF_BIAS_ALIBI if alibi else ODF_BIAS_NONE, None if slopes is None else C.addressof(slopes), softcap)
-        w = Window(min(window, _INT64_MAX), min(sinks, _INT64_MAX), q_offset)
-        nbytes = lib.odf_fwd_window_workspace_size(C.byref(p), C.byref(w))
-        ws = None
+        head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                ODF_DTYPE_BF16, ODF_DTYPE_BF16 if out.dtype is torch.bfloat16 else ODF_DTYPE_F32, B, Hq, k.shape[1], M,
+                k.shape[2], D, D, *_strides(q, "q"), *_strides(k, "k"), *_strides(v, "v"), *_strides(out, "out"),
+                1.0 / math.sqrt(D) if scale is None else scale, 1, 0, 0, 0, 0, 0,
+                ODF_BIAS_ALIBI if alibi else ODF_BIAS_NONE, 0 if slopes is None else C.addressof(slopes), softcap)
+        p = _PACK_FWD(*head, 0, 0, 0, 0, 0, 0, 0, 0)
+        w = _PACK_WINDOW(_clip(window), _clip(sinks), _clip(q_offset))
+        nbytes = lib.odf_fwd_window_workspace_size(p, w)
         if nbytes > 256:  # room for the parts of a split key range
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
-        _check(lib.odf_flash_fwd_window_sm100(C.byref(p), C.byref(w), handle))
+            p = _PACK_FWD(*head, ws.data_ptr(), nbytes, 0, 0, 0, 0, 0, 0)
+        _check(lib.odf_flash_fwd_window_sm100(p, w, handle))
     return out, (lse if want_lse else None)
 
 
@@ -399,17 +412,16 @@ def tile_map(seqlen_q, seqlen_k, causal, block_mask=None, mask_block=(128, 128),
 
 # ------------------------------------------------------------------ paged key-value cache
 # A decode step makes these calls once per layer, so they are written for few Python steps: structs are
-# filled in one constructor call, contiguous tensors pass zero strides, and the device and stream are
-# only switched where they differ from the current ones.
-_NO_STRIDES3 = (C.c_int64 * 3)()
-_NO_STRIDES2 = (C.c_int64 * 2)()
+# packed in one call, contiguous tensors pass zero strides, and the device and stream are only switched
+# where they differ from the current ones.
+_NO_STRIDES = (None, None, (0, 0), (0, 0, 0), (0, 0, 0))
 
 
 def _strides(t, name):
     """Element strides of (up to three) dimensions before the last, which must be contiguous; all zero = contiguous."""
     n = t.dim() - 1
     if t.is_contiguous():
-        return _NO_STRIDES2 if n == 2 else _NO_STRIDES3
+        return _NO_STRIDES[n]
     shape, stride = t.shape, t.stride()
     if n == 4:  # layers, which have a stride of their own
         n, shape, stride = 3, shape[1:], stride[1:]
@@ -420,7 +432,7 @@ def _strides(t, name):
         if shape[i] == 1:
             out[i] = dense
         dense *= shape[i]
-    return (C.c_int64 * n)(*out)
+    return out
 
 
 def _on(tensor, name, device):
@@ -432,7 +444,7 @@ def _int32(tensor, name, device, rows):
     """Address of a contiguous int32 device vector of `rows` elements."""
     import torch
 
-    if tensor.dtype != torch.int32 or tensor.shape != (rows,) or not tensor.is_contiguous():
+    if tensor.dtype is not torch.int32 or tensor.shape != (rows,) or not tensor.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape [{rows}], got {tensor.dtype} {list(tensor.shape)}")
     _on(tensor, name, device)
     return tensor.data_ptr()
@@ -442,7 +454,7 @@ def _scale_ptr(tensor, name, device, heads):
     import torch
 
     if tensor is None:
-        return None
+        return 0
     if tensor.dtype != torch.float32 or tensor.shape != (heads,) or not tensor.is_contiguous():
         raise ValueError(f"{name} must be a contiguous float32 tensor [{heads}]")
     _on(tensor, name, device)
@@ -450,23 +462,23 @@ def _scale_ptr(tensor, name, device, heads):
 
 
 def _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, device, batch, heads=None, head_dim=None):
-    """odf_paged_cache of one layer's pages (PagedCache), checked against the call's other tensors.  Without
+    """The values of odf_paged_cache for one layer's pages, checked against the call's other tensors.  Without
     a page table the pages may have a leading dimension of layers (page_copy)."""
     import torch
 
     shape, dtype = k_pages.shape, k_pages.dtype
     if v_pages.shape != shape or (len(shape) != 4 and (page_table is not None or len(shape) != 5)):
         raise ValueError("k_pages and v_pages must be rank 4 [pages, heads_kv, page_size, head_dim] of one shape")
-    if v_pages.dtype != dtype or dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+    if v_pages.dtype is not dtype or (dtype is not torch.bfloat16 and dtype is not torch.float8_e4m3fn):
         raise ValueError(f"a cache holds bfloat16 or float8_e4m3fn, not {dtype} and {v_pages.dtype}")
     _on(k_pages, "k_pages", device)
     _on(v_pages, "v_pages", device)
     pages, hkv, page_size, dim = shape if len(shape) == 4 else shape[1:]
     if (heads is not None and heads != hkv) or (head_dim is not None and head_dim != dim):
         raise ValueError("the new tensors and the cache must have the same kv-heads and head_dim")
-    table, table_stride, max_pages = None, 0, 0
+    table = table_stride = max_pages = 0
     if page_table is not None:
-        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
+        if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
             raise ValueError(f"page_table must be int32 [{batch}, max_pages], got {page_table.dtype} {list(page_table.shape)}")
         max_pages = page_table.shape[1]
         if not page_table.is_contiguous():
@@ -477,10 +489,10 @@ def _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, device, batch,
                 raise ValueError("page_table rows must not overlap")
         _on(page_table, "page_table", device)
         table = page_table.data_ptr()
-    return PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), ODF_DTYPE_BF16 if dtype == torch.bfloat16 else ODF_DTYPE_E4M3,
-                      pages, hkv, page_size, dim, _strides(k_pages, "k_pages"), _strides(v_pages, "v_pages"),
-                      _scale_ptr(k_scale, "k_scale", device, hkv), _scale_ptr(v_scale, "v_scale", device, hkv),
-                      table, table_stride, max_pages)
+    return (k_pages.data_ptr(), v_pages.data_ptr(), ODF_DTYPE_BF16 if dtype is torch.bfloat16 else ODF_DTYPE_E4M3,
+            pages, hkv, page_size, dim, *_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"),
+            0 if k_scale is None else _scale_ptr(k_scale, "k_scale", device, hkv),
+            0 if v_scale is None else _scale_ptr(v_scale, "v_scale", device, hkv), table, table_stride, max_pages)
 
 
 class _StayHere:
@@ -554,6 +566,11 @@ def _outputs(q, out, lse_out, out_dtype, want_lse):
     return out, lse_out
 
 
+def _clip(n):
+    """A count as the C side takes it: below zero is refused there, and past 63 bits nothing changes."""
+    return max(-1, min(n, _INT64_MAX))
+
+
 def _slopes_array(alibi_slopes, heads):
     if alibi_slopes is None:
         return None
@@ -599,15 +616,15 @@ def paged_decode(q, k_pages, v_pages, page_table, lens, *, scale=None, window=0,
     with where:
         out, lse = _outputs(q, out, lse_out, out_dtype, want_lse)
         if workspace is None:
-            workspace = paged_decode_workspace(B, Hq, cache.heads_kv, D, device=dev)
+            workspace = paged_decode_workspace(B, Hq, cache[4], D, device=dev)
         else:
             _on(workspace, "workspace", dev)
-        p = DecodeParams(q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-                         ODF_DTYPE_BF16 if out.dtype == torch.bfloat16 else ODF_DTYPE_F32, B, Hq, _strides(q, "q"),
-                         _strides(out, "out"), lens_ptr, cache, 1.0 / math.sqrt(D) if scale is None else scale,
-                         min(window, _INT64_MAX), min(sinks, _INT64_MAX), ODF_BIAS_ALIBI if alibi else ODF_BIAS_NONE,
-                         None if slopes is None else C.addressof(slopes), softcap, workspace.data_ptr(), workspace.nbytes)
-        _check(load_library().odf_paged_decode_sm100(C.byref(p), handle))
+        p = _PACK_DECODE(q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                         ODF_DTYPE_BF16 if out.dtype is torch.bfloat16 else ODF_DTYPE_F32, B, Hq, *_strides(q, "q"),
+                         *_strides(out, "out"), lens_ptr, *cache, 1.0 / math.sqrt(D) if scale is None else scale,
+                         _clip(window), _clip(sinks), ODF_BIAS_ALIBI if alibi else ODF_BIAS_NONE,
+                         0 if slopes is None else C.addressof(slopes), softcap, workspace.data_ptr(), workspace.nbytes)
+        _check(load_library().odf_paged_decode_sm100(p, handle))
     return out, (lse if want_lse else None)
 
 
@@ -626,11 +643,11 @@ def paged_append(k, v, k_pages, v_pages, page_table, starts, *, counts=None, k_s
     _require_cuda(dev)
     _on(v, "v", dev)
     cache = _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, dev, B, Hkv, D)
-    p = AppendParams(k.data_ptr(), v.data_ptr(), B, T, _strides(k, "k"), _strides(v, "v"), _int32(starts, "starts", dev, B),
-                     None if counts is None else _int32(counts, "counts", dev, B), cache)
+    p = _PACK_APPEND(k.data_ptr(), v.data_ptr(), B, T, *_strides(k, "k"), *_strides(v, "v"), _int32(starts, "starts", dev, B),
+                     0 if counts is None else _int32(counts, "counts", dev, B), *cache)
     where, handle = _launch_on(dev, stream)
     with where:
-        _check(load_library().odf_paged_append_sm100(C.byref(p), handle))
+        _check(load_library().odf_paged_append_sm100(p, handle))
 
 
 def page_copy(k_pages, v_pages, pairs, *, stream=None):
@@ -662,10 +679,10 @@ def page_copy(k_pages, v_pages, pairs, *, stream=None):
         layers, k_layer, v_layer = shape[0], k_pages.stride(0), v_pages.stride(0)
         if layers == 0:
             raise ValueError("the cache has no layers")
-    p = PageCopyParams(cache, layers, k_layer, v_layer, ids.ctypes.data, len(ids))
+    p = _PACK_COPY(*cache, layers, k_layer, v_layer, ids.ctypes.data, len(ids))
     where, handle = _launch_on(dev, stream)
     with where:
-        _check(load_library().odf_page_copy_sm100(C.byref(p), handle))
+        _check(load_library().odf_page_copy_sm100(p, handle))
 
 
 class PagePool:

@@ -229,6 +229,37 @@ def test_pool_random_against_model(seed):
             assert row == pages + [-1] * (total - len(pages))
 
 
+@pytest.mark.parametrize("pack,cls", [("_PACK_DECODE", odf.DecodeParams), ("_PACK_APPEND", odf.AppendParams),
+                                      ("_PACK_COPY", odf.PageCopyParams), ("_PACK_FWD", odf.FwdParams),
+                                      ("_PACK_WINDOW", odf.Window)])
+def test_packed_structs_are_the_ctypes_ones(pack, cls):
+    """Every field of the packed form lands where the ctypes struct (and so the C one) has it."""
+    def leaves(c):
+        for name, t in c._fields_:
+            if issubclass(t, C.Structure):
+                yield from leaves(t)
+            else:
+                n = getattr(t, "_length_", 1)
+                yield from [t._type_ if n > 1 else t] * n
+
+    values = [i + 0.5 if t is C.c_float else i + 1 for i, t in enumerate(leaves(cls))]
+    raw = getattr(odf, pack)(*values)
+    assert len(raw) == C.sizeof(cls)
+    at = iter(values)
+
+    def walk(x):
+        for name, t in x._fields_:
+            v = getattr(x, name)
+            if isinstance(v, C.Structure):
+                walk(v)
+            elif hasattr(t, "_length_"):
+                assert list(v) == [next(at) for _ in v], name
+            else:
+                assert v == next(at), name
+
+    walk(cls.from_buffer_copy(raw))
+
+
 def test_python_checks_without_a_device():
     import torch
 
