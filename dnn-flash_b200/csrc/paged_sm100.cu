@@ -19,8 +19,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Decode workspace: a counter per CTA, then two partial results per CTA.
-constexpr size_t kDecodeCounterBytes = 2048;
+// Decode workspace: three counters per CTA (one per level of a join), then two partial results per CTA.
+constexpr size_t kDecodeCounterBytes = 6144;
 
 __device__ __forceinline__ void bad_page(const PagedView& c) {
     if (c.status) atomicCAS(c.status, 0, ODF_ERR_BAD_PAGE);
@@ -81,8 +81,6 @@ constexpr int kFewItems = 4;             // up to a quarter of the CTAs: a CTA p
 constexpr int kMergeCols = 32;           // columns of O in a strip of the merge buffer
 constexpr int kMergeStride = kMergeCols + 4;  // floats: two rows are 8 banks apart
 constexpr int kMergeSlots = 16;          // strips of a warp
-constexpr int kJoin = 8;                 // pieces read at a time in a join
-constexpr int kHeld = kDecodeWarps * kMergeStride;  // pieces whose weights fit in the merge buffer
 
 template <int D, bool kE4M3, int R>
 struct DecodeCfg {
@@ -93,10 +91,11 @@ struct DecodeCfg {
     static constexpr int kSlice = kRowBytes >= 256 ? 16 : 32;
     static constexpr int kTileBytes = kSlice * kRowBytes;   // K or V of a slice
     static constexpr int kStageBytes = 2 * kTileBytes;
-    static constexpr int kCtas = R == 1 ? kCtasPerSm : 2;
     // 16 KB a warp with three CTAs of four warps on an SM, 24 KB with two: 96 or 128 KB of loads in flight
-    // behind the slices that are being computed
-    static constexpr int kStages = (R == 1 ? 16384 : 24576) / kStageBytes;
+    // behind the slices that are being computed.  8-bit rows of 128 do better with two (their conversions leave
+    // the third nothing to issue: 540 MB in 117 us against 124), 8-bit rows of 64 with three (84 against 91).
+    static constexpr int kCtas = R == 1 && !(kE4M3 && D == 128) ? kCtasPerSm : 2;
+    static constexpr int kStages = (kCtas == 3 ? 16384 : 24576) / kStageBytes;
     static constexpr int kChunks = kRowBytes / 16;          // 16-byte chunks of a row
     static constexpr int kOffMerge = kDecodeWarps * kStages * kStageBytes;
     static constexpr int kOffStats = kOffMerge + kDecodeWarps * kMergeSlots * kMergeStride * 4;
@@ -198,8 +197,9 @@ struct RunCursor {
         vis = visible_keys(a, __ldg(a.lens + b));
         n = max(1, (vis.count + kSlice - 1) / kSlice);
     }
+    bool whole;    // the run is of whole items
     __device__ __forceinline__ void cut() {
-        s1 = min(n - s0, left) + s0;
+        s1 = whole ? n : min(n - s0, left) + s0;
         left -= s1 - s0;
     }
     __device__ __forceinline__ bool next(const DecodeArgs& a) {
@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
             total = most * a.items_per_seq;
             mine = lane == 0 ? total : 0;
         } else {
+#pragma unroll 4
             for (int b = b0; b < b1; ++b) {
                 const int n = slices_of(b);
                 mine += n;
@@ -278,8 +279,10 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
             before = scan(mine, total);
         }
         const int items = a.batch * a.items_per_seq;
-        // A CTA per item when the longest is not much longer than an even share (about what streams in
-        // the time that cutting items and joining the pieces takes)
+        // No item is cut when the longest streams in about the time that cutting items and joining the pieces
+        // takes (40 slices): runs are of whole items, or, with a CTA for each, items may also be near
+        // an even share
+        const bool uncut = most <= 40;
         const bool whole_items = items <= grid && most <= total / 160 + 40;
         const bool few = whole_items || items <= grid / kFewItems;
         int at_b = 0, at_r = 0, at_s = 0;
@@ -291,8 +294,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
         } else {
             int len = 1;  // few items: slices of a piece, at most
             if (few) {
-                // an item's pieces are even, and their weights fit the merge buffer
-                len = max(max(kMinSlices, total / (grid - items) + 1), (most + kHeld - 1) / kHeld);
+                len = max(kMinSlices, total / (grid - items) + 1);  // an item's pieces are even
                 if (a.batch == 1) {
                     total = (most + len - 1) / len * a.items_per_seq;
                     mine = lane == 0 ? total : 0;
@@ -333,6 +335,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
         cur.r = at_r;
         cur.s0 = at_s;
         cur.enter(a);
+        cur.whole = false;
         if (few) {
             few_piece = at_s;
             cur.s1 = cur.n;
@@ -345,7 +348,13 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
             }
         } else {
             cur.left = runs.start(cta + 1) - first;
-            cur.cut();
+            cur.whole = uncut;
+            if (uncut && cur.s0 > 0) {  // the items that start in the run
+                cur.left -= cur.n - cur.s0;
+                if (!cur.next(a)) return;
+            } else {
+                cur.cut();
+            }
         }
     }
 
@@ -774,119 +783,109 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
             }
         }
         if (!whole) {
-            int c_first = static_cast<int>(blockIdx.x) - few_piece;
+            int index = few_piece;  // of this piece
             if (few_piece < 0) {
-                c_first = runs.owner(item0);
+                const int c_first = runs.owner(item0);
+                index = static_cast<int>(blockIdx.x) - c_first;
                 pieces = runs.owner(item0 + cur.n - 1) - c_first + 1;
             }
-            __syncthreads();  // the CTA's part is written, as seen from its first thread
+            // Joined in a tree of eights: whoever is last to finish of a group of eight pieces joins them into the slot of
+            // the group's first, then stands for the group among the next eight.  Each step waits twice (about
+            // 0.8 us) for other SMs' results: the counter, and all of the group's loads at once.
+            const int c_first = static_cast<int>(blockIdx.x) - index;
+            float* p0 = slots + 2 * static_cast<int64_t>(c_first) * kSlotFloats;  // piece k > 0: 2 k slots on
+            unsigned int* counter = static_cast<unsigned int*>(a.workspace) + c_first;
             int* last = reinterpret_cast<int*>(smem + Cfg::kOffLast);
-            if (threadIdx.x == 0) {
-                __threadfence();
-                const unsigned int old =
-                    atomicInc(static_cast<unsigned int*>(a.workspace) + c_first, static_cast<unsigned int>(pieces - 1));
-                __threadfence();
-                *last = old == static_cast<unsigned int>(pieces - 1);
-            }
-            __syncthreads();
-            if (*last != 0) {
-                // Every step here waits for L2 (about 0.5 us) and comes from a cold instruction cache, so: few
-                // steps, many loads to a step, little code.
-                const float* p0 = slots + 2 * static_cast<int64_t>(c_first) * kSlotFloats;  // piece k > 0: 2 k slots on
-                auto piece = [&](int k) { return p0 + (k == 0 ? kSlotFloats : 2 * k * kSlotFloats); };
-                auto weight = [](float mk, float mr) { return mk == -INFINITY ? 0.0f : ptx::ex2(mk - mr); };
-                float* wts = merge;  // [kHeld][kRowsMax]
-                // common max and sum, a warp to a row
-#pragma unroll 2
-                for (int r = warp; r < rows; r += kDecodeWarps) {
-                    float mj = -INFINITY, lj = 0.0f;
+            int stride = 1;
 #pragma unroll 1
-                    for (int k = lane; k < pieces; k += 32) {
-                        const float mk = __ldcg(piece(k) + kRows * D + r);
-                        const float lk = __ldcg(piece(k) + kRows * D + kRows + r);
-                        if (k < kHeld) wts[k * kRowsMax + r] = mk;
-                        const float mn = fmaxf(mj, mk);
-                        lj = lj * (mj == mn ? 1.0f : weight(mj, mn)) + lk * (mk == mn ? 1.0f : weight(mk, mn));
-                        mj = mn;
+            for (;;) {
+                const int base = index & ~7;           // the group's first piece, of `pieces` that are `stride` apart
+                const int n = min(8, pieces - base);
+                float* group = p0 + (base == 0 ? kSlotFloats : 2 * base * stride * kSlotFloats);
+                auto piece = [&](int k) { return k == 0 ? group : p0 + 2 * (base + k) * stride * kSlotFloats; };
+                if (n > 1) {
+                    __syncthreads();  // the CTA's part is written, as seen from its first thread
+                    if (threadIdx.x == 0) {
+                        __threadfence();
+                        const unsigned int old = atomicInc(counter + base * stride, static_cast<unsigned int>(n - 1));
+                        __threadfence();
+                        *last = old == static_cast<unsigned int>(n - 1);
                     }
-                    float mr = mj;
+                    __syncthreads();
+                    if (*last == 0) break;
+                    // common max and sum by row, 8 or 16 threads to a row; then the pieces' weights
+                    float* wts = merge;  // [8][kRowsMax]
+                    {
+                        constexpr int kPer = kDecodeThreads / kRows;
+                        const int r = threadIdx.x / kPer, sub = threadIdx.x % kPer;
+                        float mk = -INFINITY, lk = 0.0f;
+                        if (sub < n) {
+                            mk = __ldcg(piece(sub) + kRows * D + r);
+                            lk = __ldcg(piece(sub) + kRows * D + kRows + r);
+                        }
+                        float mr = mk;
 #pragma unroll
-                    for (int off = 16; off > 0; off >>= 1) mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, off));
-                    lj *= mj == mr ? 1.0f : weight(mj, mr);
+                        for (int off = 4; off > 0; off >>= 1) mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, off));
+                        const float w = mk == -INFINITY ? 0.0f : ptx::ex2(mk - mr);
+                        lk *= w;
 #pragma unroll
-                    for (int off = 16; off > 0; off >>= 1) lj += __shfl_xor_sync(0xffffffffu, lj, off);
-#pragma unroll 1
-                    for (int k = lane; k < min(pieces, kHeld); k += 32)
-                        wts[k * kRowsMax + r] = weight(wts[k * kRowsMax + r], mr);
-                    if (lane == 0) {
-                        stat_m[r] = mr;
-                        stat_l[r] = lj;
-                        write_lse(r, mr, lj);
-                    }
-                }
-                __syncthreads();
-                // O in float4 units of the rows, two to a thread; with few rows the pieces are spread over
-                // groups of threads too
-                const int units = rows * (D / 4);
-                const int groups = max(1, kDecodeThreads / units);
-                const int grp = static_cast<int>(threadIdx.x) / units;
-                const int u_first = groups > 1 ? static_cast<int>(threadIdx.x) - grp * units : static_cast<int>(threadIdx.x);
-#pragma unroll 1
-                for (int u0 = u_first; u0 < units; u0 += 2 * kDecodeThreads) {
-                    const int u1 = min(u0 + kDecodeThreads, units - 1);
-                    const bool two = u0 + kDecodeThreads < units;
-                    float4 x0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), x1 = x0;
-                    if (groups == 1 || grp < groups) {
-#pragma unroll 1
-                        for (int k0 = groups > 1 ? grp : 0; k0 < pieces; k0 += kJoin * groups) {
-                            float4 y0[kJoin], y1[kJoin];
-#pragma unroll
-                            for (int i = 0; i < kJoin; ++i) {
-                                const float4* pk = reinterpret_cast<const float4*>(piece(min(k0 + i * groups, pieces - 1)));
-                                y0[i] = __ldcg(pk + u0);
-                                y1[i] = y0[i];
-                                if (two) y1[i] = __ldcg(pk + u1);
-                            }
-#pragma unroll
-                            for (int i = 0; i < kJoin; ++i) {
-                                const int k = k0 + i * groups;
-                                float w0 = 0.0f, w1 = 0.0f;
-                                if (k < pieces && pieces <= kHeld) {
-                                    w0 = wts[k * kRowsMax + u0 / (D / 4)];
-                                    w1 = wts[k * kRowsMax + u1 / (D / 4)];
-                                } else if (k < pieces) {  // one item over most of the GPU
-                                    w0 = weight(__ldcg(piece(k) + kRows * D + u0 / (D / 4)), stat_m[u0 / (D / 4)]);
-                                    w1 = weight(__ldcg(piece(k) + kRows * D + u1 / (D / 4)), stat_m[u1 / (D / 4)]);
-                                }
-                                x0.x += w0 * y0[i].x;
-                                x0.y += w0 * y0[i].y;
-                                x0.z += w0 * y0[i].z;
-                                x0.w += w0 * y0[i].w;
-                                x1.x += w1 * y1[i].x;
-                                x1.y += w1 * y1[i].y;
-                                x1.z += w1 * y1[i].z;
-                                x1.w += w1 * y1[i].w;
-                            }
+                        for (int off = 4; off > 0; off >>= 1) lk += __shfl_xor_sync(0xffffffffu, lk, off);
+                        if (sub < 8) wts[sub * kRowsMax + r] = w;
+                        if (sub == 0) {
+                            stat_m[r] = mr;
+                            stat_l[r] = lk;
                         }
                     }
-                    if (groups > 1) {
-                        __syncthreads();  // the weights have been read
-                        float4* sums = reinterpret_cast<float4*>(merge);
-                        if (grp < groups) sums[threadIdx.x] = x0;
-                        __syncthreads();
+                    __syncthreads();
+                    // O in float4 units of the rows, two to a thread
+                    const int units = rows * (D / 4);
 #pragma unroll 1
-                        for (int k = 1; k < groups && grp == 0; ++k) {
-                            const float4 y = sums[k * units + u0];
-                            x0.x += y.x;
-                            x0.y += y.y;
-                            x0.z += y.z;
-                            x0.w += y.w;
+                    for (int u0 = threadIdx.x; u0 < units; u0 += 2 * kDecodeThreads) {
+                        const int u1 = u0 + kDecodeThreads;
+                        float4 y0[8], y1[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float4* pk = reinterpret_cast<const float4*>(piece(min(k, n - 1)));
+                            y0[k] = __ldcg(pk + u0);
+                            y1[k] = u1 < units ? __ldcg(pk + u1) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         }
-                        if (grp != 0) break;
+                        const int r0 = u0 / (D / 4), r1 = min(u1, units - 1) / (D / 4);
+                        float4 x0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), x1 = x0;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float w0 = k < n ? wts[k * kRowsMax + r0] : 0.0f;
+                            const float w1 = k < n ? wts[k * kRowsMax + r1] : 0.0f;
+                            x0.x += w0 * y0[k].x;
+                            x0.y += w0 * y0[k].y;
+                            x0.z += w0 * y0[k].z;
+                            x0.w += w0 * y0[k].w;
+                            x1.x += w1 * y1[k].x;
+                            x1.y += w1 * y1[k].y;
+                            x1.z += w1 * y1[k].z;
+                            x1.w += w1 * y1[k].w;
+                        }
+                        if (pieces <= 8) {
+                            write_out(r0, (u0 % (D / 4)) * 4, x0, stat_l[r0]);
+                            if (u1 < units) write_out(r1, (u1 % (D / 4)) * 4, x1, stat_l[r1]);
+                        } else {
+                            reinterpret_cast<float4*>(group)[u0] = x0;
+                            if (u1 < units) reinterpret_cast<float4*>(group)[u1] = x1;
+                        }
                     }
-                    write_out(u0 / (D / 4), (u0 % (D / 4)) * 4, x0, stat_l[u0 / (D / 4)]);
-                    if (two) write_out(u1 / (D / 4), (u1 % (D / 4)) * 4, x1, stat_l[u1 / (D / 4)]);
+                    if (threadIdx.x < rows) {
+                        if (pieces <= 8) {
+                            write_lse(threadIdx.x, stat_m[threadIdx.x], stat_l[threadIdx.x]);
+                        } else {
+                            group[kRows * D + threadIdx.x] = stat_m[threadIdx.x];
+                            group[kRows * D + kRows + threadIdx.x] = stat_l[threadIdx.x];
+                        }
+                    }
                 }
+                if (pieces <= 8) break;
+                counter += kDecodeMaxCtas;  // a row of counters per level
+                index >>= 3;
+                pieces = (pieces + 7) >> 3;
+                stride <<= 3;
             }
             __syncthreads();  // before the next piece writes what was read here
         }
@@ -1129,7 +1128,8 @@ cudaError_t set_paged_kernel_attrs() {
 }
 
 int launch_paged_decode(DecodeArgs& a, int32_t head_dim, int32_t kv_dtype, cudaStream_t stream, const char** err) {
-    static_assert(kDecodeCounterBytes >= kDecodeMaxCtas * sizeof(unsigned int), "a counter per CTA");
+    static_assert(kDecodeCounterBytes >= 3 * kDecodeMaxCtas * sizeof(unsigned int), "three counters per CTA");
+    static_assert(kDecodeMaxCtas <= 512, "three levels of eights");
     a.k16_page = static_cast<uint32_t>(a.c.k_page / 16);
     a.k16_head = static_cast<uint32_t>(a.c.k_head / 16);
     a.k16_slot = static_cast<uint32_t>(a.c.k_slot / 16);
