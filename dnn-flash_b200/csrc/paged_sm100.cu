@@ -77,6 +77,7 @@ constexpr int kDecodeMaxCtas = kCtasPerSm * 148;
 constexpr int kRowsMax = 16;             // query heads of an item, at most
 constexpr int kMinSlices = 16;           // fewest slices worth a CTA of their own
 constexpr int kAhead = 2;                // slices whose page ids are asked for before their load
+constexpr int kItemCost = 8;             // slices that stream in the time an item takes besides: Q, joining, output
 constexpr int kFewItems = 4;             // up to a quarter of the CTAs: a CTA per piece
 constexpr int kMergeCols = 32;           // columns of O in a strip of the merge buffer
 constexpr int kMergeStride = kMergeCols + 4;  // floats: two rows are 8 banks apart
@@ -174,11 +175,11 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Runs of `total` slices: the first `more` CTAs have one slice more than the others' `len`.
+// Runs of equal length: the first `more` CTAs' are one longer than the others' `len`.
 struct Runs {
     int len, more;
     __device__ __forceinline__ int start(int cta) const { return cta * len + min(cta, more); }
-    // the CTA whose run holds slice s
+    // the CTA whose run holds s
     __device__ __forceinline__ int owner(int s) const {
         const int edge = more * (len + 1);
         return s < edge ? static_cast<int>(static_cast<uint32_t>(s) / static_cast<uint32_t>(len + 1))
@@ -186,32 +187,35 @@ struct Runs {
     }
 };
 
-// Walks a CTA's run piece by piece: slices [s0, s1) of item r of sequence b.
+// Walks a CTA's run piece by piece: slices [s0, s1) of item r of sequence b.  Runs are measured in slices plus
+// kItemCost per item, spent before its first slice.
 template <int kSlice>
 struct RunCursor {
     int b, r, s0, s1;
-    int left;      // slices of the run after this piece
+    int left;      // of the run after this piece
+    bool whole;    // the run is of whole items
     Visible vis;
     int n;         // slices of the item: one at least, so that an empty one is written too
     __device__ __forceinline__ void enter(const DecodeArgs& a) {
         vis = visible_keys(a, __ldg(a.lens + b));
         n = max(1, (vis.count + kSlice - 1) / kSlice);
     }
-    bool whole;    // the run is of whole items
-    __device__ __forceinline__ void cut() {
-        s1 = whole ? n : min(n - s0, left) + s0;
-        left -= s1 - s0;
+    // the piece from offset x of the item on; false if the run ends before a slice of it
+    __device__ __forceinline__ bool cut(int x) {
+        const int end = whole ? n + kItemCost : min(n + kItemCost, x + left);
+        left -= end - x;
+        s0 = max(0, x - kItemCost);
+        s1 = max(0, end - kItemCost);
+        return s1 > s0;
     }
     __device__ __forceinline__ bool next(const DecodeArgs& a) {
         if (left <= 0) return false;
-        s0 = 0;
         if (++r == a.items_per_seq) {
             r = 0;
             ++b;
             enter(a);
         }
-        cut();
-        return true;
+        return cut(0);
     }
 };
 
@@ -241,7 +245,8 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
     // ---- the run of this CTA; every warp works it out for itself, a lane per batch / 32 sequences
     RunCursor<kSlice> cur;
     Runs runs{0, 0};
-    int first = 0;                   // number of this CTA's first slice
+    int first = 0;                   // where this CTA's run starts
+    int item0 = 0;                   // and its item
     int few_piece = -1, pieces = 0;  // a CTA per piece: which piece of its item this one has, of how many
     {
         const int cta = static_cast<int>(blockIdx.x), grid = static_cast<int>(gridDim.x);
@@ -306,17 +311,20 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
                 if (cta >= total) return;
                 first = cta;
             } else {
-                const int ctas = min(grid, (total + kMinSlices - 1) / kMinSlices);
+                total += kItemCost * items;
+                mine += kItemCost * (b1 - b0) * a.items_per_seq;
+                before += kItemCost * b0 * a.items_per_seq;
+                const int ctas = min(grid, (total + kMinSlices + kItemCost - 1) / (kMinSlices + kItemCost));
                 if (cta >= ctas) return;
                 runs.len = total / ctas;
                 runs.more = total - runs.len * ctas;
                 first = runs.start(cta);
             }
-            // the lane whose sequences hold `first` finds the item and the slice (or piece) in it
+            // the lane whose sequences hold `first` finds the item and the place (or piece) in it
             const bool here = first >= before && first < before + mine;
             if (here) {
                 for (at_b = b0;; ++at_b) {
-                    const int n = (slices_of(at_b) + len - 1) / len;
+                    const int n = few ? (slices_of(at_b) + len - 1) / len : slices_of(at_b) + kItemCost;
                     if (first < before + n * a.items_per_seq) {
                         at_r = static_cast<int>(static_cast<uint32_t>(first - before) / static_cast<uint32_t>(n));
                         at_s = first - before - at_r * n;
@@ -349,11 +357,12 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
         } else {
             cur.left = runs.start(cta + 1) - first;
             cur.whole = uncut;
-            if (uncut && cur.s0 > 0) {  // the items that start in the run
-                cur.left -= cur.n - cur.s0;
+            item0 = first - at_s;
+            if (uncut && at_s > 0) {  // the items that start in the run
+                cur.left -= cur.n + kItemCost - at_s;
                 if (!cur.next(a)) return;
-            } else {
-                cur.cut();
+            } else if (!cur.cut(at_s)) {
+                return;
             }
         }
     }
@@ -431,7 +440,6 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
     for (int i = 0; i < kStages - 1; ++i) load();
 
     int slot = 0;  // ring slot of the next slice to compute
-    int item0 = first - cur.s0;  // number of the item's first slice
     for (;;) {
         const int hk = cur.r / a.row_tiles;
         const int row0 = (cur.r - hk * a.row_tiles) * kRows;  // first query head of the item, within the group
@@ -785,9 +793,9 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
         if (!whole) {
             int index = few_piece;  // of this piece
             if (few_piece < 0) {
-                const int c_first = runs.owner(item0);
+                const int c_first = runs.owner(item0 + kItemCost);
                 index = static_cast<int>(blockIdx.x) - c_first;
-                pieces = runs.owner(item0 + cur.n - 1) - c_first + 1;
+                pieces = runs.owner(item0 + kItemCost + cur.n - 1) - c_first + 1;
             }
             // Joined in a tree of eights: whoever is last to finish of a group of eight pieces joins them into the slot of
             // the group's first, then stands for the group among the next eight.  Each step waits twice (about
@@ -889,7 +897,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
             }
             __syncthreads();  // before the next piece writes what was read here
         }
-        item0 += cur.n;
+        item0 += cur.n + kItemCost;
         if (!cur.next(a)) break;
     }
     cp_async_wait<0>();
@@ -1094,7 +1102,7 @@ cudaError_t launch_decode(DecodeArgs& a, cudaStream_t stream, const char** err) 
     const int64_t keys = a.window > 0 ? std::min<int64_t>(room, static_cast<int64_t>(a.window) + a.sinks) : room;
     const int64_t items = static_cast<int64_t>(a.items_per_seq) * a.batch;
     const int64_t slices = (keys + Cfg::kSlice - 1) / Cfg::kSlice;
-    if (slices * items > 0x7fffffffLL) {  // the kernel counts them in 32 bits
+    if ((slices + kItemCost) * items > 0x7fffffffLL) {  // the kernel counts them in 32 bits
         *err = "batch x kv-heads x the page table's room is beyond the kernel's 32 bits";
         return cudaErrorNotSupported;
     }

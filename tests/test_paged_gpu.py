@@ -86,8 +86,11 @@ def test_decode(case, kv):
 def test_decode_random_batches(kv, D):
     """Many sequences of every length: work split over the cache's length and over sequences."""
     g = torch.Generator().manual_seed(D)
-    for B, hi, Hkv, group, page in ((1, 30000, 2, 3, 16), (5, 6000, 4, 8, 64), (70, 900, 2, 5, 16), (300, 60, 3, 1, 8)):
+    for B, hi, Hkv, group, page in ((1, 30000, 2, 3, 16), (5, 6000, 4, 8, 64), (70, 900, 2, 5, 16), (300, 60, 3, 1, 8),
+                                    (200, 20, 4, 2, 16), (90, 5000, 3, 12, 16)):
         lens = torch.randint(0, hi, (B,), generator=g).tolist()
+        if hi == 20:
+            lens[77], lens[140] = 9000, 1400  # two long ones among many short
         cache = ref.Cache(lens, Hkv=Hkv, D=D, page=page, kv=kv, seed=B)
         q = _q(B, Hkv * group, D, seed=B)
         o, lse = _decode(cache, q, out_dtype=torch.bfloat16)
