@@ -3,6 +3,8 @@ from __future__ import annotations
 
 import ctypes as C
 import random
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -82,6 +84,26 @@ def test_append_refuses(field, value, code):
     lib = odf.load_library()
     assert lib.odf_paged_append_sm100(C.byref(_append(**{field: value})), None) == code
     assert odf.last_error()
+
+
+def test_decode_refuses_what_does_not_fit_its_counters():
+    """Explicit slopes past 256 heads, a K pool past 64 GB."""
+    lib = odf.load_library()
+    slopes = (C.c_float * 300)()
+    p = _decode(heads_q=300, bias_kind=odf.ODF_BIAS_ALIBI, alibi_slopes=C.cast(slopes, C.c_void_p))
+    assert lib.odf_paged_decode_sm100(C.byref(p), None) == UNS and "256" in odf.last_error()
+    p = _decode(**{"cache.num_pages": 1 << 24, "cache.k_strides": (4096, 1024, 64)})
+    assert lib.odf_paged_decode_sm100(C.byref(p), None) == UNS and "64 GB" in odf.last_error()
+
+
+def test_headers_compile_as_c(tmp_path):
+    src = tmp_path / "use.c"
+    src.write_text('#include "odf_paged_sm100.h"\n#include "odf_sm100.h"\n'
+                   "int main(void) { odf_decode_params p = {0}; odf_window w = {1, 0, 0};\n"
+                   "  return (int)(p.batch + w.sinks) + ODF_ERR_NO_PAGES - 8; }\n")
+    include = Path(__file__).resolve().parents[1] / "include"
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Wextra", "-Werror", f"-I{include}", "-c", "-o", str(tmp_path / "use.o"),
+                    str(src)], check=True)
 
 
 def test_null_params():

@@ -126,6 +126,35 @@ def test_decode_nonfinite_where_visible():
     assert torch.isfinite(o).all() and torch.isfinite(lse).all()
 
 
+def test_decode_many_heads_with_generated_slopes():
+    """More heads than explicit slopes may have: the kernel works them out itself."""
+    cache = ref.Cache([300, 20], Hkv=40, D=64, page=16, seed=12)
+    q = _q(2, 320, 64)
+    o, lse = _decode(cache, q, alibi=True, out_dtype=torch.bfloat16)
+    ref.check_decode(o, lse, q, cache, slopes=odf.alibi_slopes(320))
+
+
+def test_decode_shared_pages_and_repeated_sequences():
+    """Tables that name the same pages (a fork before it is written), one of them cut short."""
+    cache = ref.Cache([700], Hkv=2, D=128, page=16, seed=13)
+    q = _q(3, 8, 128)
+    many = ref.Cache.__new__(ref.Cache)
+    many.__dict__.update(cache.__dict__)
+    many.table = cache.table.expand(3, -1).contiguous()
+    many.lens_list = [700, 700, 333]
+    many.lens = torch.tensor(many.lens_list, dtype=torch.int32, device="cuda")
+    o, lse = _decode(many, q, out_dtype=torch.bfloat16)
+    ref.check_decode(o, lse, q, many)
+
+
+def test_decode_table_wider_than_the_lengths():
+    """Room for a million tokens, and one token: what the table could hold is no work."""
+    cache = ref.Cache([1, 0, 40], Hkv=2, D=64, page=16, seed=14, max_pages=65536)
+    q = _q(3, 4, 64)
+    o, lse = _decode(cache, q)
+    ref.check_decode(o, lse, q, cache)
+
+
 def test_decode_strided_and_given_outputs():
     lens = [500, 20]
     cache = ref.Cache(lens, Hkv=2, D=128, page=16, seed=8, max_pages=40)

@@ -1,7 +1,11 @@
 """Sliding-window attention with sinks on the GPU against a 64-bit reference."""
 from __future__ import annotations
 
+import json
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -158,6 +162,19 @@ def test_long_prompt_sampled_rows():
     o, lse = odf.flash_fwd_window(q, k, v, window=4096, sinks=4, out_dtype=torch.bfloat16)
     rows = torch.tensor([0, 1, 4095, 4096, 4099, 4100, 20000, 32767], device="cuda")
     _check(o, lse, q, k, v, window=4096, sinks=4, rows=rows)
+
+
+def test_checked_build_invariants_hold():
+    """Work items, KV entries, ring loads and P.V counts of the window variants, counted in the kernel."""
+    root = Path(__file__).resolve().parent.parent
+    assert (root / "dnn-flash_b200" / "lib" / "libodf_sm100_checked.so").exists()
+    proc = subprocess.run([sys.executable, str(root / "tests" / "checked_window_run.py")], capture_output=True, text=True,
+                          timeout=600)
+    assert proc.returncode == 0, proc.stderr[-3000:]
+    results = [json.loads(line) for line in proc.stdout.splitlines() if line.startswith("{")]
+    assert len(results) == 6
+    for r in results:
+        assert r["rc"] == 0 and r["check_bits"] == 0 and r["status"] == 0, r
 
 
 # ------------------------------------------------------------------------------------- together
