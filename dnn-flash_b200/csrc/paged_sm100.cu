@@ -64,8 +64,8 @@ __device__ __forceinline__ Visible visible_keys(const DecodeArgs& a, int len) {
 // the lengths, by a prefix sum over the lengths that every warp does for itself; when items are
 // few, or their lengths near enough, each has CTAs of its own.  A run holds pieces of one or several
 // items; an item that lies in one run is written out directly, the pieces of one that does not go
-// to the workspace as fp32 O, max and sum, and the CTA that is last to finish (a counter that
-// wraps to zero) joins them in order, so the result does not depend on who that is.
+// to the workspace as fp32 O, max and sum, and are joined by whichever CTA is last to finish of each group of
+// eight (counters that wrap to zero), in an order that does not depend on who that is.
 //
 // Inside a piece the warps take slices in turn, each with a softmax of its own (running max and sum,
 // O in registers) and a ring of its own in shared memory, filled by cp.async kStages - 1 slices
@@ -75,7 +75,8 @@ constexpr int kDecodeThreads = kDecodeWarps * 32;
 constexpr int kCtasPerSm = 3;            // of one block of query heads; two of two blocks
 constexpr int kDecodeMaxCtas = kCtasPerSm * 148;
 constexpr int kRowsMax = 16;             // query heads of an item, at most
-constexpr int kMinSlices = 16;           // fewest slices worth a CTA of their own
+constexpr int kMinSlices = 8;            // fewest slices worth a CTA of their own (8 sequences of 1024 keys: 13.9 us
+                                         // with 16, 12.5 with 8; 1 of 1500: 11.3 and 12.2)
 constexpr int kAhead = 2;                // slices whose page ids are asked for before their load
 constexpr int kItemCost = 12;            // slices that stream in the time an item takes besides (Q, joining, output);
                                          // of 5, 8, 12 and 20 the best over ragged, short, e4m3 and 16-head batches
@@ -94,9 +95,9 @@ struct DecodeCfg {
     static constexpr int kTileBytes = kSlice * kRowBytes;   // K or V of a slice
     static constexpr int kStageBytes = 2 * kTileBytes;
     // 16 KB a warp with three CTAs of four warps on an SM, 24 KB with two: 96 or 128 KB of loads in flight
-    // behind the slices that are being computed.  8-bit rows of 128 do better with two (their conversions leave
-    // the third nothing to issue: 540 MB in 117 us against 124), 8-bit rows of 64 with three (84 against 91).
-    static constexpr int kCtas = R == 1 && !(kE4M3 && D == 128) ? kCtasPerSm : 2;
+    // behind the slices that are being computed.  Three do as well or better wherever their registers
+    // allow it (64 ragged sequences of 8-bit rows of 64: 57 us against 66).
+    static constexpr int kCtas = R == 1 ? kCtasPerSm : 2;
     static constexpr int kStages = (kCtas == 3 ? 16384 : 24576) / kStageBytes;
     static constexpr int kChunks = kRowBytes / 16;          // 16-byte chunks of a row
     static constexpr int kOffMerge = kDecodeWarps * kStages * kStageBytes;
@@ -213,7 +214,7 @@ struct RunCursor {
         if (left <= 0) return false;
         if (++r == a.items_per_seq) {
             r = 0;
-            ++b;
+            if (++b >= a.batch) return false;  // only with lengths that change under the kernel
             enter(a);
         }
         return cut(0);
@@ -286,10 +287,10 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
         }
         const int items = a.batch * a.items_per_seq;
         // No item is cut when the longest streams in about the time that cutting items and joining the pieces
-        // takes (40 slices): runs are of whole items, or, with a CTA for each, items may also be near
-        // an even share
+        // takes: runs are of whole items; with a CTA for each, items may also be near an even share (with 40
+        // for 24, 8 sequences of 1024 keys, 64 slices an item, take 17.4 us, cut 12.5)
         const bool uncut = most <= 40;
-        const bool whole_items = items <= grid && most <= total / 160 + 40;
+        const bool whole_items = items <= grid && most <= total / 160 + 24;
         const bool few = whole_items || items <= grid / kFewItems;
         int at_b = 0, at_r = 0, at_s = 0;
         if (whole_items) {
@@ -324,15 +325,14 @@ __global__ void __launch_bounds__(kDecodeThreads, DecodeCfg<D, kE4M3, R>::kCtas)
             // the lane whose sequences hold `first` finds the item and the place (or piece) in it
             const bool here = first >= before && first < before + mine;
             if (here) {
-                for (at_b = b0;; ++at_b) {
+                for (at_b = b0; at_b < b1 - 1; ++at_b) {
                     const int n = few ? (slices_of(at_b) + len - 1) / len : slices_of(at_b) + kItemCost;
-                    if (first < before + n * a.items_per_seq) {
-                        at_r = static_cast<int>(static_cast<uint32_t>(first - before) / static_cast<uint32_t>(n));
-                        at_s = first - before - at_r * n;
-                        break;
-                    }
+                    if (first < before + n * a.items_per_seq) break;
                     before += n * a.items_per_seq;
                 }
+                const int n = few ? (slices_of(at_b) + len - 1) / len : slices_of(at_b) + kItemCost;
+                at_r = min(a.items_per_seq - 1, static_cast<int>(static_cast<uint32_t>(first - before) / static_cast<uint32_t>(n)));
+                at_s = first - before - at_r * n;
             }
             const int who = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
             at_b = __shfl_sync(0xffffffffu, at_b, who);
