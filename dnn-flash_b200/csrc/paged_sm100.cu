@@ -57,7 +57,9 @@ __device__ __forceinline__ Visible visible_keys(const DecodeArgs& a, int len) {
 // Products are warp-level m16n8k16 with the keys as the 16 rows: S^T = K Q^T, then O^T += V^T P^T, the
 // query heads of one kv-head as the 8 columns (one block of them up to 8 heads, else two).  tcgen05 would
 // want 128 rows of keys by 8 columns through tensor memory; the warp-level product leaves the tensor
-// pipe a quarter busy and needs no hand-over between warps.
+// pipe 9% busy (16% with an 8-bit cache) and needs no hand-over between warps.
+//
+// 64 sequences of up to 8192 keys, 64/8 heads: 1075 MB in 163 us, 6.6 TB/s; one of 129 keys 4.3 us.
 //
 // Work: an item is (sequence, kv-head, block of query heads); its visible keys are cut into slices of 16 or
 // 32.  The slices of all items in a row are dealt to the CTAs in equal consecutive runs, whatever

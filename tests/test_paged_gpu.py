@@ -174,6 +174,29 @@ def test_decode_strided_and_given_outputs():
     ref.check_decode(o, None, q, cache)
 
 
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_decode_and_append_with_unlike_layouts(kv):
+    """K as [page, head, slot], V as [page, slot, head] with a gap between rows; the pages inside a larger pool."""
+    cache = ref.Cache([333, 50, 7], Hkv=3, D=64, page=16, kv=kv, seed=21)
+    pages = cache.k.shape[0]
+    wide = torch.zeros((2 * pages, 16, 3, 64 + 32), device="cuda").to(cache.v.dtype)
+    v = wide[::2, :, :, :64].transpose(1, 2)
+    v.copy_(cache.v)
+    cache.v = v
+    q = _q(3, 9, 64)
+    o, lse = _decode(cache, q)
+    ref.check_decode(o, lse, q, cache)
+    k = torch.randn((3, 3, 2, 64), device="cuda").to(torch.bfloat16)
+    before = wide.float()
+    odf.paged_append(k, k, cache.k, cache.v, cache.table, torch.tensor([3, 0, 5], device="cuda", dtype=torch.int32),
+                     k_scale=cache.ks, v_scale=cache.vs)
+    got = cache.v[int(cache.table[0, 0]), :, 3:5].float()
+    want = k[0].float() if kv == "bf16" else ref.to_e4m3((k[0].float() / cache.vs.view(-1, 1, 1)).double()).float()
+    assert torch.equal(got, want)
+    assert torch.equal(torch.nan_to_num(wide[1::2].float()), torch.nan_to_num(before[1::2]))
+    assert torch.equal(wide[..., 64:].float(), before[..., 64:])
+
+
 def test_decode_beyond_32_bits():
     """Pages whose byte offsets need more than 32 bits."""
     Hkv, D, page = 8, 128, 64
