@@ -325,9 +325,9 @@ def flash_fwd_window(q, k, v, *, window, sinks=0, q_offset=0, scale=None, alibi=
     slopes = _slopes_array(alibi_slopes, Hq) if alibi else None
     where, handle = _launch_on(dev, stream)
     with where:
-        out, lse = _outputs(q, out, lse_out, out_dtype, want_lse)
+        out, lse, o_code = _outputs(q, out, lse_out, out_dtype, want_lse, B, Hq, M)
         head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                ODF_DTYPE_BF16, ODF_DTYPE_BF16 if out.dtype is torch.bfloat16 else ODF_DTYPE_F32, B, Hq, k.shape[1], M,
+                ODF_DTYPE_BF16, o_code, B, Hq, k.shape[1], M,
                 k.shape[2], D, D, *_strides(q, "q"), *_strides(k, "k"), *_strides(v, "v"), *_strides(out, "out"),
                 1.0 / math.sqrt(D) if scale is None else scale, 1, 0, 0, 0, 0, 0,
                 ODF_BIAS_ALIBI if alibi else ODF_BIAS_NONE, 0 if slopes is None else C.addressof(slopes), softcap)
@@ -444,9 +444,10 @@ def _int32(tensor, name, device, rows):
     """Address of a contiguous int32 device vector of `rows` elements."""
     import torch
 
-    if tensor.dtype is not torch.int32 or tensor.shape != (rows,) or not tensor.is_contiguous():
+    if (tensor.dtype is not torch.int32 or tensor.shape != (rows,) or not tensor.is_contiguous()
+            or tensor.device != device):
+        _on(tensor, name, device)
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape [{rows}], got {tensor.dtype} {list(tensor.shape)}")
-    _on(tensor, name, device)
     return tensor.data_ptr()
 
 
@@ -464,35 +465,54 @@ def _scale_ptr(tensor, name, device, heads):
 def _cache_params(k_pages, v_pages, k_scale, v_scale, page_table, device, batch, heads=None, head_dim=None):
     """The values of odf_paged_cache for one layer's pages, checked against the call's other tensors.  Without
     a page table the pages may have a leading dimension of layers (page_copy)."""
-    import torch
-
-    shape, dtype = k_pages.shape, k_pages.dtype
-    if v_pages.shape != shape or (len(shape) != 4 and (page_table is not None or len(shape) != 5)):
-        raise ValueError("k_pages and v_pages must be rank 4 [pages, heads_kv, page_size, head_dim] of one shape")
-    if v_pages.dtype is not dtype or (dtype is not torch.bfloat16 and dtype is not torch.float8_e4m3fn):
-        raise ValueError(f"a cache holds bfloat16 or float8_e4m3fn, not {dtype} and {v_pages.dtype}")
-    _on(k_pages, "k_pages", device)
-    _on(v_pages, "v_pages", device)
+    shape = k_pages.shape
+    kind = _cache_kind(k_pages.dtype)
+    if (kind is None or v_pages.dtype is not k_pages.dtype or v_pages.shape != shape or k_pages.device != device
+            or v_pages.device != device or len(shape) not in (4, 5) or (len(shape) == 5 and page_table is not None)):
+        raise _bad_cache(k_pages, v_pages, device)
     pages, hkv, page_size, dim = shape if len(shape) == 4 else shape[1:]
     if (heads is not None and heads != hkv) or (head_dim is not None and head_dim != dim):
         raise ValueError("the new tensors and the cache must have the same kv-heads and head_dim")
     table = table_stride = max_pages = 0
     if page_table is not None:
-        if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
+        rows, max_pages = page_table.shape if page_table.dim() == 2 else (-1, 0)
+        if rows != batch or page_table.dtype is not _int32_dtype or page_table.device != device:
+            _on(page_table, "page_table", device)
             raise ValueError(f"page_table must be int32 [{batch}, max_pages], got {page_table.dtype} {list(page_table.shape)}")
-        max_pages = page_table.shape[1]
         if not page_table.is_contiguous():
             if page_table.stride(1) != 1 and max_pages > 1:
                 raise ValueError("page_table must be contiguous in its last dimension")
             table_stride = page_table.stride(0) if batch > 1 else 0
             if batch > 1 and table_stride < max_pages:  # rows that overlap, an expanded table among them
                 raise ValueError("page_table rows must not overlap")
-        _on(page_table, "page_table", device)
         table = page_table.data_ptr()
-    return (k_pages.data_ptr(), v_pages.data_ptr(), ODF_DTYPE_BF16 if dtype is torch.bfloat16 else ODF_DTYPE_E4M3,
-            pages, hkv, page_size, dim, *_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"),
+    return (k_pages.data_ptr(), v_pages.data_ptr(), kind, pages, hkv, page_size, dim,
+            *(_NO_STRIDES[3] if k_pages.is_contiguous() else _strides(k_pages, "k_pages")),
+            *(_NO_STRIDES[3] if v_pages.is_contiguous() else _strides(v_pages, "v_pages")),
             0 if k_scale is None else _scale_ptr(k_scale, "k_scale", device, hkv),
             0 if v_scale is None else _scale_ptr(v_scale, "v_scale", device, hkv), table, table_stride, max_pages)
+
+
+_cache_kinds = _int32_dtype = None
+
+
+def _cache_kind(dtype):
+    global _cache_kinds, _int32_dtype
+    if _cache_kinds is None:
+        import torch
+
+        _cache_kinds = {torch.bfloat16: ODF_DTYPE_BF16, torch.float8_e4m3fn: ODF_DTYPE_E4M3}
+        _int32_dtype = torch.int32
+    return _cache_kinds.get(dtype)
+
+
+def _bad_cache(k_pages, v_pages, device):
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if t.device != device:
+            return ValueError(f"{name} is on {t.device}, the call runs on {device}")
+    if k_pages.dtype != v_pages.dtype or _cache_kind(k_pages.dtype) is None:
+        return ValueError(f"a cache holds bfloat16 or float8_e4m3fn, not {k_pages.dtype} and {v_pages.dtype}")
+    return ValueError("k_pages and v_pages must be rank 4 [pages, heads_kv, page_size, head_dim] of one shape")
 
 
 class _StayHere:
@@ -543,8 +563,8 @@ def _require_cuda(device):
         raise ValueError(f"tensors must be on a CUDA device, not {device}")
 
 
-def _outputs(q, out, lse_out, out_dtype, want_lse):
-    """The given or new outputs of an attention call with q's shape."""
+def _outputs(q, out, lse_out, out_dtype, want_lse, *lead):
+    """The given or new outputs of an attention call with q's shape [*lead, D], and out's dtype code."""
     import torch
 
     if out is None:
@@ -558,12 +578,13 @@ def _outputs(q, out, lse_out, out_dtype, want_lse):
         _on(out, "out", q.device)
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise ValueError("out must be float32 or bfloat16")
+    code = ODF_DTYPE_BF16 if dtype is torch.bfloat16 else ODF_DTYPE_F32
     if lse_out is None:
-        return out, q.new_empty(*q.shape[:-1], dtype=torch.float32) if want_lse else None
+        return out, q.new_empty(*lead, dtype=torch.float32) if want_lse else None, code
     _on(lse_out, "lse_out", q.device)
-    if lse_out.shape != q.shape[:-1] or lse_out.dtype != torch.float32 or not lse_out.is_contiguous():
+    if lse_out.shape != lead or lse_out.dtype != torch.float32 or not lse_out.is_contiguous():
         raise ValueError("lse_out must be contiguous float32 of q's shape without its last dimension")
-    return out, lse_out
+    return out, lse_out, code
 
 
 def _clip(n):
@@ -614,14 +635,14 @@ def paged_decode(q, k_pages, v_pages, page_table, lens, *, scale=None, window=0,
     slopes = _slopes_array(alibi_slopes, Hq) if alibi else None
     where, handle = _launch_on(dev, stream)
     with where:
-        out, lse = _outputs(q, out, lse_out, out_dtype, want_lse)
+        out, lse, o_code = _outputs(q, out, lse_out, out_dtype, want_lse, B, Hq)
         if workspace is None:
             workspace = paged_decode_workspace(B, Hq, cache[4], D, device=dev)
         else:
             _on(workspace, "workspace", dev)
         p = _PACK_DECODE(q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                         ODF_DTYPE_BF16 if out.dtype is torch.bfloat16 else ODF_DTYPE_F32, B, Hq, *_strides(q, "q"),
-                         *_strides(out, "out"), lens_ptr, *cache, 1.0 / math.sqrt(D) if scale is None else scale,
+                         o_code, B, Hq, *(_NO_STRIDES[2] if q.is_contiguous() else _strides(q, "q")),
+                         *(_NO_STRIDES[2] if out.is_contiguous() else _strides(out, "out")), lens_ptr, *cache, 1.0 / math.sqrt(D) if scale is None else scale,
                          _clip(window), _clip(sinks), ODF_BIAS_ALIBI if alibi else ODF_BIAS_NONE,
                          0 if slopes is None else C.addressof(slopes), softcap, workspace.data_ptr(), workspace.nbytes)
         _check(load_library().odf_paged_decode_sm100(p, handle))
