@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 import os
 import struct
 from pathlib import Path
@@ -327,8 +328,7 @@ def flash_fwd_window(q, k, v, *, window, sinks=0, q_offset=0, scale=None, alibi=
     with where:
         out, lse, o_code = _outputs(q, out, lse_out, out_dtype, want_lse, B, Hq, M)
         head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                ODF_DTYPE_BF16, o_code, B, Hq, k.shape[1], M,
-                k.shape[2], D, D, *_strides(q, "q"), *_strides(k, "k"), *_strides(v, "v"), *_strides(out, "out"),
+                ODF_DTYPE_BF16, o_code, B, Hq, k.shape[1], M, k.shape[2], D, D, *_strides(q, "q"), *_strides(k, "k"), *_strides(v, "v"), *_strides(out, "out"),
                 1.0 / math.sqrt(D) if scale is None else scale, 1, 0, 0, 0, 0, 0,
                 ODF_BIAS_ALIBI if alibi else ODF_BIAS_NONE, 0 if slopes is None else C.addressof(slopes), softcap)
         p = _PACK_FWD(*head, 0, 0, 0, 0, 0, 0, 0, 0)
@@ -642,7 +642,8 @@ def paged_decode(q, k_pages, v_pages, page_table, lens, *, scale=None, window=0,
             _on(workspace, "workspace", dev)
         p = _PACK_DECODE(q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
                          o_code, B, Hq, *(_NO_STRIDES[2] if q.is_contiguous() else _strides(q, "q")),
-                         *(_NO_STRIDES[2] if out.is_contiguous() else _strides(out, "out")), lens_ptr, *cache, 1.0 / math.sqrt(D) if scale is None else scale,
+                         *(_NO_STRIDES[2] if out.is_contiguous() else _strides(out, "out")), lens_ptr, *cache,
+                         1.0 / math.sqrt(D) if scale is None else scale,
                          _clip(window), _clip(sinks), ODF_BIAS_ALIBI if alibi else ODF_BIAS_NONE,
                          0 if slopes is None else C.addressof(slopes), softcap, workspace.data_ptr(), workspace.nbytes)
         _check(load_library().odf_paged_decode_sm100(p, handle))
@@ -671,6 +672,31 @@ def paged_append(k, v, k_pages, v_pages, page_table, starts, *, counts=None, k_s
         _check(load_library().odf_paged_append_sm100(p, handle))
 
 
+def _page_ids(pairs, n, pages):
+    """The ids of n pairs as an int32 array (and its address), checked before they are cut to 32 bits."""
+    if n <= 32:  # a few: plain Python is 3 us faster than numpy
+        rows = pairs.tolist() if hasattr(pairs, "tolist") else pairs
+        try:
+            flat = [operator.index(i) for src, dst in rows for i in (src, dst)]
+        except (TypeError, ValueError):
+            raise ValueError("pairs must be integers of shape [n, 2]") from None
+        if min(flat) < 0 or max(flat) >= pages:
+            raise ValueError("a page id is outside the cache")
+        ids = (C.c_int32 * (2 * n))(*flat)
+        return ids, C.addressof(ids)
+    import numpy as np
+
+    ids = np.asarray(pairs)
+    if ids.ndim != 2 or ids.shape[1] != 2 or ids.dtype.kind not in "iu":
+        raise ValueError("pairs must be integers of shape [n, 2]")
+    if ids.dtype != np.int32:
+        ids = np.ascontiguousarray(ids, dtype=np.int64)
+        if ids.view(np.uint64).max() >= pages:  # negative ids are large here
+            raise ValueError("a page id is outside the cache")
+    ids = np.ascontiguousarray(ids, dtype=np.int32)
+    return ids, ids.ctypes.data
+
+
 def page_copy(k_pages, v_pages, pairs, *, stream=None):
     """Copies pages pairs[i] = (source, destination) of K and V (odf_page_copy_sm100).
 
@@ -678,32 +704,25 @@ def page_copy(k_pages, v_pages, pairs, *, stream=None):
     launch.  ``pairs``: a sequence of pairs, a numpy array or a CPU tensor [n,2], such as
     ``PagePool`` gives out.  Asynchronous on ``stream``.
     """
-    import numpy as np
-
     rank, shape, dev = k_pages.dim(), k_pages.shape, k_pages.device
     if rank not in (4, 5) or v_pages.shape != shape:
         raise ValueError("k_pages and v_pages must be [pages, Hkv, page_size, D] or [layers, pages, ...] of one shape")
     _require_cuda(dev)
-    ids = np.asarray(pairs)
-    if ids.size == 0:
+    n = len(pairs)
+    if n == 0:
         return
-    if ids.ndim != 2 or ids.shape[1] != 2 or ids.dtype.kind not in "iu":
-        raise ValueError("pairs must be integers of shape [n, 2]")
-    if ids.dtype != np.int32:
-        ids = np.ascontiguousarray(ids, dtype=np.int64)
-        if ids.view(np.uint64).max() >= shape[-4]:  # before they are cut to 32 bits; negative ids are large here
-            raise ValueError("a page id is outside the cache")
-    ids = np.ascontiguousarray(ids, dtype=np.int32)
+    ids, address = _page_ids(pairs, n, shape[-4])
     cache = _cache_params(k_pages, v_pages, None, None, None, dev, 0)
     layers, k_layer, v_layer = 1, 0, 0
     if rank == 5:
         layers, k_layer, v_layer = shape[0], k_pages.stride(0), v_pages.stride(0)
         if layers == 0:
             raise ValueError("the cache has no layers")
-    p = _PACK_COPY(*cache, layers, k_layer, v_layer, ids.ctypes.data, len(ids))
+    p = _PACK_COPY(*cache, layers, k_layer, v_layer, address, n)
     where, handle = _launch_on(dev, stream)
     with where:
         _check(load_library().odf_page_copy_sm100(p, handle))
+    del ids  # held until the call has read them
 
 
 class PagePool:

@@ -395,8 +395,17 @@ def test_refusals_of_the_binding():
                  dict(lse_out=torch.empty((2, 3), device="cuda"))):
         with pytest.raises(ValueError):
             odf.paged_decode(**{**ok, **over})
-    with pytest.raises(ValueError, match="outside"):
-        odf.page_copy(cache.k, cache.v, [(0, cache.k.shape[0])])
+    for n in (1, 40):  # few and many pairs take different ways
+        for bad in ((0, cache.k.shape[0]), (-1, 0), (0, 2 ** 32 + 1)):
+            with pytest.raises(ValueError, match="outside"):
+                odf.page_copy(cache.k, cache.v, [bad] * n)
+            with pytest.raises(ValueError, match="outside"):
+                odf.page_copy(cache.k, cache.v, torch.tensor([bad] * n))
+        for bad in ([(0, 1, 2)] * n, [0] * n, torch.rand(n, 2), [(0.5, 1)] * n):
+            with pytest.raises(ValueError, match="integers"):
+                odf.page_copy(cache.k, cache.v, bad)
+        with pytest.raises(ValueError, match="read" if n == 1 else "twice"):
+            odf.page_copy(cache.k, cache.v, [(0, 0)] * n)
 
 
 # ------------------------------------------------------------------------------------- together
