@@ -56,6 +56,9 @@ typedef struct odf_paged_cache {
  * with mod the ALiBi term slope[h] * (j - p) and the soft-cap of odf_fwd_params.  lens[b] <= 0
  * writes o = 0, lse = -inf.  K and V of keys that are not visible, and slots past a sequence's
  * end, may hold anything, NaN included.  Accumulation and softmax are fp32.
+ * Limits (ODF_ERR_UNSUPPORTED past them): K pages, and V pages, of one layer span at most 64 GB; batch x
+ * kv-heads x the table's room is at most 2^31 slices of 16 keys; 256 explicit slopes.  Lengths must not change
+ * while a call runs.  Results do not depend on timing: the same call gives the same bits.
  */
 typedef struct odf_decode_params {
     const void* q;              /* bf16 [batch, heads_q, head_dim] */
