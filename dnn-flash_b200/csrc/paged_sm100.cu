@@ -79,7 +79,8 @@ constexpr int kDecodeMaxCtas = kCtasPerSm * 148;
 constexpr int kRowsMax = 16;             // query heads of an item, at most
 constexpr int kMinSlices = 8;            // fewest slices worth a CTA of their own (8 sequences of 1024 keys: 13.9 us
                                          // with 16, 12.5 with 8; 1 of 1500: 11.3 and 12.2)
-constexpr int kAhead = 2;                // slices whose page ids are asked for before their load
+constexpr int kAhead = 2;                // slices whose page ids are asked for before their load (3: level, 3-9% slower
+                                         // with an 8-bit cache)
 constexpr int kItemCost = 12;            // slices that stream in the time an item takes besides (Q, joining, output);
                                          // of 5, 8, 12 and 20 the best over ragged, short, e4m3 and 16-head batches
 constexpr int kFewItems = 4;             // up to a quarter of the CTAs: a CTA per piece
@@ -120,7 +121,7 @@ __device__ __forceinline__ int swizzle(int r) {
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
