@@ -105,6 +105,17 @@ def test_window_of_everything_is_the_causal_forward():
     assert (o - o2).abs().max() <= bound and (lse - lse2).abs().max() <= 1e-4
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("scale", [0.0, -0.1, 0.5, 3.0])
+def test_scales_and_far_apart_scores(D, scale):
+    """Scores that spread over hundreds (the running max moves late and often), or fall with the scale's sign."""
+    q, k, v = _qkv(1, 4, 2, 1200, 1200, D, seed=5)
+    k[:, :, 700:720] *= 8.0  # a few keys far above the others, in the middle of the windows
+    for sinks in (0, 3):
+        o, lse = odf.flash_fwd_window(q, k, v, window=500, sinks=sinks, scale=scale)
+        _check(o, lse, q, k, v, window=500, sinks=sinks, scale=scale, what=f"scale {scale} sinks {sinks}")
+
+
 def test_strides_given_outputs_and_a_side_stream():
     B, H, M, D = 2, 4, 400, 128
     q, k, v = (torch.randn((B, M, H, D), device="cuda").to(torch.bfloat16).transpose(1, 2) for _ in range(3))
