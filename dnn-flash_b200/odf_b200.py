@@ -431,6 +431,8 @@ def _strides(t, name):
     for i in range(n - 1, -1, -1):  # a dimension of size 1 has no stride of its own: a contiguous tensor's
         if shape[i] == 1:
             out[i] = dense
+        elif out[i] == 0:  # with every dimension broadcast, the C side would read zeros as a contiguous tensor's
+            raise ValueError(f"{name} is broadcast in dimension {i}, which the kernels do not take (make it contiguous)")
         dense *= shape[i]
     return out
 

@@ -1,0 +1,32 @@
+"""Strides that the binding hands to the C side, where all zero means contiguous: a tensor whose every leading
+dimension is broadcast has those strides without being contiguous, and must not get through as one."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import odf_b200 as odf
+
+
+@pytest.mark.parametrize("sizes", [(4, 8), (2, 1, 5), (4, 8, 16), (1, 1, 7), (2, 4, 8, 16)])
+def test_broadcast_tensors_are_refused(sizes):
+    x = torch.zeros(128, dtype=torch.bfloat16).expand(*sizes, 128)
+    with pytest.raises(ValueError, match="broadcast"):
+        odf._strides(x, "q")
+
+
+def test_partly_broadcast_tensors_are_refused():
+    x = torch.zeros((4, 1, 16, 64), dtype=torch.bfloat16).expand(4, 3, 16, 64)
+    with pytest.raises(ValueError, match="k is broadcast in dimension 1"):
+        odf._strides(x, "k")
+
+
+def test_strides_of_usual_tensors_stand():
+    x = torch.zeros((2, 16, 3, 64), dtype=torch.bfloat16)
+    assert tuple(odf._strides(x, "x")) == (0, 0, 0)  # contiguous
+    assert odf._strides(x.transpose(1, 2), "x") == [16 * 3 * 64, 64, 3 * 64]
+    assert odf._strides(x[:, ::2], "x") == [16 * 3 * 64, 2 * 3 * 64, 64]
+    one = torch.zeros((1, 3, 1, 128), dtype=torch.bfloat16)[..., :64]  # dimensions of one element have no stride
+    assert odf._strides(one, "x") == [3 * 64, 128, 64]
+    layers = torch.zeros((2, 5, 3, 16, 96), dtype=torch.bfloat16)[..., :64]
+    assert odf._strides(layers, "x") == [3 * 16 * 96, 16 * 96, 96]
