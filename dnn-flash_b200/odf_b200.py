@@ -200,6 +200,8 @@ def _strides4(t):
     s = t.stride()
     if s[3] != 1:
         raise ValueError("the innermost (feature) dimension must be contiguous")
+    if s[0] == s[1] == s[2] == 0 and max(t.shape[:3]) > 1:  # the C side would read zeros as a contiguous tensor's
+        raise ValueError("q, k, v and out must not be broadcast (make them contiguous)")
     return (s[0], s[1], s[2])
 
 

@@ -30,3 +30,22 @@ def test_strides_of_usual_tensors_stand():
     assert odf._strides(one, "x") == [3 * 64, 128, 64]
     layers = torch.zeros((2, 5, 3, 16, 96), dtype=torch.bfloat16)[..., :64]
     assert odf._strides(layers, "x") == [3 * 16 * 96, 16 * 96, 96]
+
+
+def _fill(q, k, v, o, bias=None):
+    return odf.fill_params(q, k, v, o, None, causal=False, scale=0.125, block_mask=None, mask_block=(128, 128), alibi=False,
+                           alibi_slopes_host=None, softcap=0.0, workspace=None, visits=None, bias=bias)[0]
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_forward_refuses_broadcast_tensors(which):
+    ts = [torch.zeros((2, 4, 8, 64), dtype=torch.bfloat16) for _ in range(4)]
+    _fill(*ts)
+    ts[which] = torch.zeros(64, dtype=torch.bfloat16).expand(2, 4, 8, 64)
+    with pytest.raises(ValueError, match="broadcast"):
+        _fill(*ts)
+
+
+def test_forward_takes_one_row():
+    ts = [torch.zeros(64, dtype=torch.bfloat16).expand(1, 1, 1, 64) for _ in range(4)]
+    _fill(*ts)
