@@ -242,9 +242,12 @@ def fill_params(q, k, v, o, lse, *, causal, scale, block_mask, mask_block, alibi
             raise ValueError("ALiBi and a bias tensor are exclusive (one BiasKind per call)")
         # float32 CUDA tensor broadcastable to [B, Hq, M, N]; expand() gives 0 strides
         bias_v = bias.expand(B, Hq, M, N)
+        strides = bias_v.stride()
+        if not any(strides):  # one value for every score: all zero means contiguous on the C side, so a row of it
+            bias_v, strides = bias_v[0, 0, 0].contiguous(), (0, 0, 0, 1)
         p.bias_kind = ODF_BIAS_SAME_SHAPE
         p.bias = bias_v.data_ptr()
-        for i, st in enumerate(bias_v.stride()):
+        for i, st in enumerate(strides):
             p.bias_strides[i] = st
         keep.append(bias_v)
     if workspace is not None:
@@ -295,10 +298,13 @@ def flash_fwd(q, k, v, *, causal=False, scale=None, block_mask=None, mask_block=
     current = torch.cuda.current_stream(dev).cuda_stream
     if stream is None:
         stream = current
+    bias_row = bias is not None and p.bias != bias.data_ptr()  # made above, on the current stream
+    if bias_row and stream != current:
+        torch.cuda.current_stream(dev).synchronize()
     _check(lib.odf_flash_fwd_sm100(C.byref(p), C.c_void_p(stream)))
     # Temporaries come from torch's allocator on the current stream; on another
     # stream they must outlive the launch, so wait for it before releasing them.
-    if stream != current and (ws is not None or mask_t is not None):
+    if stream != current and (ws is not None or mask_t is not None or bias_row):
         torch.cuda.synchronize(dev)
     del keep
     return out, (lse if want_lse else None)
@@ -383,9 +389,12 @@ def flash_fwd_host(q, k, v, *, causal=False, scale=None, block_mask=None, mask_b
     if bias is not None:  # float32 array broadcastable to [B, Hq, M, N]
         bias_v = np.broadcast_to(np.asarray(bias, dtype=np.float32), (B, Hq, M, N))
         p.bias_kind = ODF_BIAS_SAME_SHAPE
+        strides = [st // 4 for st in bias_v.strides]
+        if not any(strides):  # one value for every score, as in fill_params
+            bias_v, strides = np.ascontiguousarray(bias_v[0, 0, 0]), (0, 0, 0, 1)
         p.bias = bias_v.ctypes.data
-        for i, st in enumerate(bias_v.strides):
-            p.bias_strides[i] = st // 4
+        for i, st in enumerate(strides):
+            p.bias_strides[i] = st
     _check(lib.odf_flash_fwd_host(C.byref(p)))
     del bias_v
     return out, lse_out

@@ -2,6 +2,8 @@
 dimension is broadcast has those strides without being contiguous, and must not get through as one."""
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 import torch
 
@@ -49,3 +51,26 @@ def test_forward_refuses_broadcast_tensors(which):
 def test_forward_takes_one_row():
     ts = [torch.zeros(64, dtype=torch.bfloat16).expand(1, 1, 1, 64) for _ in range(4)]
     _fill(*ts)
+
+
+@pytest.mark.parametrize("M,N", [(8, 24), (1, 24), (8, 1), (1, 1)])
+def test_forward_bias_of_one_value(M, N):
+    """Strides that stay inside what holds the value: 0 over rows, 1 over a row of N copies."""
+    q, o = (torch.zeros((2, 4, M, 64), dtype=torch.bfloat16) for _ in range(2))
+    k, v = (torch.zeros((2, 4, N, 64), dtype=torch.bfloat16) for _ in range(2))
+    for bias in (torch.tensor(2.5), torch.full((1, 1, 1, 1), 2.5), torch.tensor([2.5]).expand(2, 4, M, N)):
+        p, keep = odf.fill_params(q, k, v, o, None, causal=False, scale=0.125, block_mask=None, mask_block=(128, 128),
+                                  alibi=False, alibi_slopes_host=None, softcap=0.0, workspace=None, visits=None, bias=bias)
+        strides = list(p.bias_strides)
+        assert any(strides) and all(s == 0 or n == 1 for s, n in zip(strides[:3], (2, 4, M)))
+        held = (C.c_float * (1 + (N - 1) * strides[3])).from_address(p.bias)
+        assert list(held) == [2.5] * len(held) and (N == 1 or strides[3] <= 1)
+        del keep
+
+
+def test_forward_bias_strides_stand():
+    q, k, v, o = (torch.zeros((2, 4, 8, 64), dtype=torch.bfloat16) for _ in range(4))
+    for shape, strides in (((1, 1, 1, 8), [0, 0, 0, 1]), ((2, 1, 1, 1), [1, 0, 0, 0]), ((1, 4, 8, 8), [0, 64, 8, 1])):
+        bias = torch.zeros(shape)
+        p = _fill(q, k, v, o, bias)
+        assert list(p.bias_strides) == strides and p.bias == bias.data_ptr()
