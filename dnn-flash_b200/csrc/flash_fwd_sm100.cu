@@ -189,7 +189,7 @@ struct RowItem {
     int split;         // which split (0 without KV splits)
     int n_full;        // sliding window: how many tiles from n_entries on are visible as a whole,
     int win_end, win_n;  // the end of this query tile's tiles and the number of the pair's
-    int pad;
+    int win_base;        // where the pair's tiles count from (WindowSpan)
 };
 static_assert(sizeof(RowItem) == 64, "RowItem layout");
 
@@ -221,15 +221,19 @@ struct Item {
     bool valid1;       // Q1 has rows
     int split, kv0;    // KV split of the item and its first KV tile (0, 0 without splits)
     int win_lo, n_sink, win_n;  // sliding window: first key of its tiles, the sink tiles before them, all tiles
+    int win_base;               // and where they count from
 };
 
 // Sliding window.  Row qi sits at position p = q_offset + qi and sees the keys j <= p with
 // p - j < window or j < sinks.  A pair of query tiles visits n_sink tiles over the sinks, if its
-// window starts past them, then tiles of 128 keys from win_lo, the first key that its first row
+// window starts past them, then tiles of 128 keys from lo, the first key that its first row
 // sees: tiles start where the window does, not at multiples of 128, so a window of W keys costs
-// ceil((W + 255) / 128) tiles and no key that every row has behind it is read.
+// ceil((W + 255) / 128) tiles and no key that every row has behind it is read.  Nor is one that every
+// row has ahead: where keys of later rows follow the pair's own (they may hold NaN, and 0 times NaN in the
+// P.V product is NaN), tile u >= 1 starts at base + 128 u, which makes the last one end at the pair's last
+// row, and of tile 0, which still starts at lo, the columns that tile 1 has are masked.
 struct WindowSpan {
-    int lo, n_sink, n_win;
+    int lo, base, n_sink, n_win;  // base in (lo - 128, lo]
 };
 
 __device__ __forceinline__ WindowSpan window_span(const FwdArgs& a, int q00, int qend) {
@@ -245,6 +249,7 @@ __device__ __forceinline__ WindowSpan window_span(const FwdArgs& a, int q00, int
             w.lo = 0;  // the window touches the sinks: one run of tiles from key 0
     }
     w.n_win = hi > w.lo ? (hi - w.lo + kTileK - 1) / kTileK : 0;
+    w.base = hi < min(a.n, a.q_offset + a.m) ? hi - w.n_win * kTileK : w.lo;  // (else the K and V maps end at hi)
     return w;
 }
 
@@ -257,8 +262,8 @@ __device__ __forceinline__ int window_tile(int j, int n) {
     return kAlibi ? n - 1 - j : j;
 }
 // First key of the pair's tile t.
-__device__ __forceinline__ int window_tile_start(int t, int lo, int n_sink) {
-    return t < n_sink ? t * kTileK : lo + (t - n_sink) * kTileK;
+__device__ __forceinline__ int window_tile_start(int t, int lo, int base, int n_sink) {
+    return t < n_sink ? t * kTileK : max(lo, base + (t - n_sink) * kTileK);
 }
 // The pair's tiles that a query tile with rows at positions [p0, pe) visits: all up to (not including) `end`,
 // but `skip`: the first window tile, which lies before the window of every row of Q1 (unless the run starts at
@@ -266,10 +271,10 @@ __device__ __forceinline__ int window_tile_start(int t, int lo, int n_sink) {
 struct WindowVisit {
     int end, skip;
 };
-__device__ __forceinline__ WindowVisit window_visit(const FwdArgs& a, int lo, int n_sink, int p0, int pe) {
+__device__ __forceinline__ WindowVisit window_visit(const FwdArgs& a, int lo, int base, int n_sink, int p0, int pe) {
     WindowVisit v;
-    v.end = n_sink + max(0, (min(a.n, pe) - lo + kTileK - 1) / kTileK);
-    v.skip = lo > 0 && p0 - a.window + 1 >= lo + kTileK ? n_sink : -1;
+    v.end = n_sink + max(0, (min(a.n, pe) - base + kTileK - 1) / kTileK);
+    v.skip = lo > 0 && p0 - a.window + 1 >= base + kTileK ? n_sink : -1;
     return v;
 }
 
@@ -352,6 +357,7 @@ __device__ __forceinline__ Item decode_item(const FwdArgs& a, int64_t k) {
     if constexpr ((MOD & kModWindow) != 0) {
         const WindowSpan w = window_span(a, I.q00, I.qend1);
         I.win_lo = w.lo;
+        I.win_base = w.base;
         I.n_sink = w.n_sink;
         I.win_n = w.n_sink + w.n_win;
         I.n_entries = I.win_n;
@@ -372,8 +378,8 @@ template <int MOD>
 __device__ __forceinline__ uint32_t kv_entry(const FwdArgs& a, const Item& I, int j) {
     if constexpr ((MOD & kModWindow) != 0) {
         const int t = window_tile<(MOD & kModAlibi) != 0>(I.kv0 + j, I.win_n);
-        const WindowVisit v0 = window_visit(a, I.win_lo, I.n_sink, a.q_offset + I.q00, a.q_offset + I.qend0);
-        const WindowVisit v1 = window_visit(a, I.win_lo, I.n_sink, a.q_offset + I.q01, a.q_offset + I.qend1);
+        const WindowVisit v0 = window_visit(a, I.win_lo, I.win_base, I.n_sink, a.q_offset + I.q00, a.q_offset + I.qend0);
+        const WindowVisit v1 = window_visit(a, I.win_lo, I.win_base, I.n_sink, a.q_offset + I.q01, a.q_offset + I.qend1);
         uint32_t e = static_cast<uint32_t>(t);
         if (t < v0.end && t != v0.skip) e |= kNeed0;
         if (I.valid1 && t < v1.end && t != v1.skip) e |= kNeed1;
@@ -591,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int j = 0; ok && j < I.n_entries; ++j) {
                         const int kt = static_cast<int>(kv_entry<MOD>(args, I, j) & 0xFFFFu);
                         int row0 = kt * kTileK;  // first key of the tile
-                        if constexpr (kWin) row0 = window_tile_start(kt, I.win_lo, I.n_sink);
+                        if constexpr (kWin) row0 = window_tile_start(kt, I.win_lo, I.win_base, I.n_sink);
 #ifdef ODF_CHECKED
                         {
                             const uint32_t e_chk = kv_entry<MOD>(args, I, j);
@@ -894,16 +900,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (kWin) {
                     const int p0 = args.q_offset + r.q0;
                     const WindowVisit v =
-                        window_visit(args, I.win_lo, I.n_sink, p0, args.q_offset + min(args.m, r.q0 + kTileQ));
+                        window_visit(args, I.win_lo, I.win_base, I.n_sink, p0, args.q_offset + min(args.m, r.q0 + kTileQ));
                     r.n_iter = valid ? I.n_entries : 0;
                     r.pair = v.skip;
                     r.win_end = v.end;
                     r.win_n = I.win_n;
+                    r.win_base = I.win_base;
                     // tiles [full, full + n_full) of the window are visible as a whole to this warp's rows
                     const int wp0 = p0 + (warp & 3) * 32;
-                    const int seen = min(wp0 + 1, args.n) - I.win_lo;  // keys that the first row reaches, from win_lo on
-                    const int first = args.sinks >= args.n ? 0 : max(0, wp0 + 32 - args.window - I.win_lo);
-                    const int full = (first + kTileK - 1) / kTileK;
+                    const int seen = min(wp0 + 1, args.n) - I.win_base;  // keys that the first row reaches, from base on
+                    const int first = args.sinks >= args.n ? 0 : max(0, wp0 + 32 - args.window - I.win_base);
+                    const int full = max(I.win_base < I.win_lo ? 1 : 0, (first + kTileK - 1) / kTileK);
                     r.n_entries = I.n_sink + full;
                     r.n_full = max(0, (seen < 0 ? 0 : seen / kTileK) - full);
                 } else if (args.mode == kModeList) {
@@ -957,19 +964,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // sliding window, for this warp's 32 rows at positions [wp0, wp0 + 31]: every key
                 // of the tile visible, no key visible, some rows' window starting inside it
                 bool win_full = false, win_none = false, win_low = false;
+                int k_end = 0;  // the end of the tile's keys (sliding window)
                 if constexpr (kWin) {
                     const int64_t span = rec->bias_off;
                     const int n_sink = static_cast<int>(span >> 32);
                     kt = window_tile<(MOD & kModAlibi) != 0>(rec->kv0 + j, rec->win_n);
                     if (kt == rec->pair || kt >= rec->win_end) continue;
                     sink_tile = kt < n_sink;
-                    k0 = window_tile_start(kt, static_cast<int>(span), n_sink);
+                    k0 = window_tile_start(kt, static_cast<int>(span), rec->win_base, n_sink);
+                    k_end = sink_tile ? args.sinks : rec->win_base + (kt - n_sink + 1) * kTileK;
                     win_full = static_cast<uint32_t>(kt - rec->n_entries) < static_cast<uint32_t>(rec->n_full);
                     if (!win_full) {
                         const int wp0 = args.q_offset + q0 + wq * 32;
                         win_full = sink_tile && k0 + kTileK <= args.sinks;
                         win_low = !sink_tile && k0 <= wp0 + 31 - args.window;
-                        win_none = !sink_tile && (k0 > wp0 + 31 || (k0 >= args.sinks && k0 + kTileK - 1 <= wp0 - args.window));
+                        win_none = !sink_tile && (k0 > wp0 + 31 || (k0 >= args.sinks && k_end - 1 <= wp0 - args.window));
                     }
                 }
                 // Waits are per thread; the warp re-converges (and agrees) before the
@@ -1211,10 +1220,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // cover a disallowed BlockMask block, its bit in the row's 128-bit allow mask.
                 if constexpr (kWin) {
                     if (!win_full) {
-                        // columns [0, limit] that exist and are not ahead of the row (in a sink
-                        // tile: that are sinks), of them those in its window or among the sinks
-                        int limit = min(args.n - 1, pos) - k0;
-                        if (sink_tile) limit = min(limit, args.sinks - 1 - k0);
+                        // columns [0, limit] that exist, are the tile's own (in a sink tile: sinks) and are not
+                        // ahead of the row, of them those in its window or among the sinks
+                        const int limit = min(min(args.n, k_end) - 1, pos) - k0;
                         if (!win_low) {
 #pragma unroll
                             for (int c = 0; c < 128; ++c) s[c] = (c <= limit) ? s[c] : -INFINITY;

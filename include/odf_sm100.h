@@ -124,7 +124,7 @@ size_t odf_fwd_workspace_size(const odf_fwd_params* p);
  * see later keys); block masks, bias tensors and tile_visits are refused (ODF_ERR_UNSUPPORTED).
  * Rows that see nothing get 0 and LSE -inf.  Keys that no row of the call sees may hold anything, NaN
  * included (evicted pages, room for tokens to come); a non-finite value in a key that some row does see
- * can reach other rows of its 256-row block.
+ * can reach the outputs of all rows of a 256-row block (counted from row 0) that has such a row, and of no others.
  * The token-exact counterpart of the block mask in attention.hpp:20-29, which a window that is
  * not a multiple of its block size cannot be written as.
  */
