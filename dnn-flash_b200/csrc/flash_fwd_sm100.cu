@@ -1432,8 +1432,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (valid_row && args.lse) {
                     const float m_use = (m_run == -INFINITY) ? 0.0f : m_run;
+                    // -inf says that the row sees no key; in the sliding-window variants a sum of NaN stays NaN
+                    const bool none = kWin ? l_run == 0.0f : !(l_run > 0.0f);
                     args.lse[static_cast<int64_t>(rec->split) * args.lse_split + static_cast<int64_t>(rec->bh) * args.m + qi] =
-                        (l_run > 0.0f) ? (m_use + log2f(l_run)) * kLn2 : -INFINITY;
+                        none ? -INFINITY : (m_use + log2f(l_run)) * kLn2;
                 }
             }
         }
@@ -1743,7 +1745,7 @@ cudaError_t launch_d(const CUtensorMap& tq, const CUtensorMap& tk, const CUtenso
 // Merge of the KV splits' partial results, one warp per (batch, q-head, query row): with the
 // splits' natural-log LSE_s and normalised O_s, LSE = log sum_s exp(LSE_s) and
 // O = sum_s exp(LSE_s - LSE) O_s (splits with LSE_s = -inf, no key of the row in them, weigh 0;
-// a row with no key at all gets O = 0 and LSE = -inf, as without splits).
+// a row with no key at all gets O = 0 and LSE = -inf, as without splits).  A NaN among them stays NaN.
 template <int D>
 __global__ void __launch_bounds__(256) split_combine_kernel(const float* __restrict__ po, const float* __restrict__ pl,
                                                             int n_splits, int64_t o_split, int64_t l_split,
@@ -1755,9 +1757,15 @@ __global__ void __launch_bounds__(256) split_combine_kernel(const float* __restr
     if (row >= rows) return;  // whole warps leave together
     // the splits' LSEs, lane l holding splits l, l + 32, ...: the row's max, then its weight sum
     float mx = -INFINITY;
-    for (int sp = lane; sp < n_splits; sp += 32) mx = fmaxf(mx, __ldg(pl + sp * l_split + row));
+    bool nan = false;
+    for (int sp = lane; sp < n_splits; sp += 32) {
+        const float l = __ldg(pl + sp * l_split + row);
+        mx = fmaxf(mx, l);
+        nan |= isnan(l);
+    }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    if (__any_sync(0xffffffffu, nan)) mx = NAN;  // fmaxf drops it
     float acc[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = 0.0f;
