@@ -173,6 +173,13 @@ int odf_paged_decode_sm100(const odf_decode_params* p, void* stream) {
     if (a.q_b <= 0 || a.q_h <= 0 || a.o_b <= 0 || a.o_h <= 0 || a.q_b % 8 || a.q_h % 8 || (a.o_b * oes) % 16 ||
         (a.o_h * oes) % 16)
         return set_error(ODF_ERR_INVALID_ARG, "q and o strides must be positive multiples of 16 bytes (or all zero for contiguous)");
+    a.batch = static_cast<int32_t>(p->batch);
+    a.heads_q = static_cast<int32_t>(p->heads_q);
+    a.group = static_cast<int32_t>(p->heads_q / p->cache.heads_kv);
+    a.window = static_cast<int32_t>(std::min<int64_t>(p->window, 0x7fffffff));
+    a.sinks = static_cast<int32_t>(std::min<int64_t>(p->sinks, 0x7fffffff));
+    if (!odf::decode_work_fits(a, static_cast<int32_t>(D), p->cache.kv_dtype))
+        return set_error(ODF_ERR_UNSUPPORTED, "batch x kv-heads x the page table's room is beyond the kernel's 32 bits");
     if (p->workspace == nullptr || p->workspace_bytes < odf_paged_decode_workspace_size(p))
         return set_error(ODF_ERR_INVALID_ARG, "the workspace is smaller than odf_paged_decode_workspace_size() bytes");
     if (!aligned(p->workspace, 16)) return set_error(ODF_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
@@ -184,14 +191,9 @@ int odf_paged_decode_sm100(const odf_decode_params* p, void* stream) {
     a.lse = p->lse;
     a.lens = p->lens;
     a.o_bf16 = p->o_dtype == ODF_DTYPE_BF16;
-    a.batch = static_cast<int32_t>(p->batch);
-    a.heads_q = static_cast<int32_t>(p->heads_q);
-    a.group = static_cast<int32_t>(p->heads_q / p->cache.heads_kv);
     a.scale = p->scale;
     a.softcap = p->softcap;
     a.inv_softcap = p->softcap > 0.0f ? 1.0f / p->softcap : 0.0f;
-    a.window = static_cast<int32_t>(std::min<int64_t>(p->window, 0x7fffffff));
-    a.sinks = static_cast<int32_t>(std::min<int64_t>(p->sinks, 0x7fffffff));
     a.has_alibi = p->bias_kind == ODF_BIAS_ALIBI;
     if (a.has_alibi) {
         if (p->alibi_slopes != nullptr) {

@@ -71,6 +71,9 @@ struct CopyArgs {
     int64_t n_pairs;
 };
 
+// Whether the slices of a decode call, as the kernel counts them, stay within its 32 bits (no CUDA call).  Reads the
+// cache's sizes, batch, group, window and sinks.
+bool decode_work_fits(const DecodeArgs& a, int32_t head_dim, int32_t kv_dtype);
 int launch_paged_decode(DecodeArgs& a, int32_t head_dim, int32_t kv_dtype, cudaStream_t stream, const char** err);
 int launch_paged_append(AppendArgs& a, int32_t head_dim, int32_t kv_dtype, cudaStream_t stream, const char** err);
 int launch_page_copy(const CopyArgs& a, cudaStream_t stream, const char** err);

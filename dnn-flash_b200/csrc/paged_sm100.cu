@@ -1109,21 +1109,22 @@ size_t decode_workspace_bytes(int32_t head_dim) {
 
 namespace {
 
+// Most keys that a sequence of this call can have visible.
+int64_t decode_keys(const DecodeArgs& a) {
+    const int64_t room = static_cast<int64_t>(a.c.max_pages) * a.c.page_size;
+    return a.window > 0 ? std::min<int64_t>(room, static_cast<int64_t>(a.window) + a.sinks) : room;
+}
+
 template <int D, bool kE4M3, int R>
-cudaError_t launch_decode(DecodeArgs& a, cudaStream_t stream, const char** err) {
+cudaError_t launch_decode(DecodeArgs& a, cudaStream_t stream) {
     using Cfg = DecodeCfg<D, kE4M3, R>;
     a.row_tiles = (a.group + Cfg::kRows - 1) / Cfg::kRows;
     a.items_per_seq = a.c.heads_kv * a.row_tiles;
     a.fd_items = make_fastdiv(static_cast<uint32_t>(a.items_per_seq));
     // no more CTAs than the page table's room could give work to, but one for every piece of few items
-    const int64_t room = static_cast<int64_t>(a.c.max_pages) * a.c.page_size;
-    const int64_t keys = a.window > 0 ? std::min<int64_t>(room, static_cast<int64_t>(a.window) + a.sinks) : room;
+    const int64_t keys = decode_keys(a);
     const int64_t items = static_cast<int64_t>(a.items_per_seq) * a.batch;
     const int64_t slices = (keys + Cfg::kSlice - 1) / Cfg::kSlice;
-    if ((slices + kItemCost) * items > 0x7fffffffLL) {  // the kernel counts them in 32 bits
-        *err = "batch x kv-heads x the page table's room is beyond the kernel's 32 bits";
-        return cudaErrorNotSupported;
-    }
     const int64_t worth = std::max((slices + kMinSlices - 1) / kMinSlices, static_cast<int64_t>(kFewItems)) * items;
     const int64_t most = std::min<int64_t>(Cfg::kCtas * 148, static_cast<int64_t>(Cfg::kCtas) * a.sm_count);
     const unsigned grid = static_cast<unsigned>(std::min(most, worth));
@@ -1132,11 +1133,30 @@ cudaError_t launch_decode(DecodeArgs& a, cudaStream_t stream, const char** err) 
 }
 
 template <int D, bool kE4M3>
-cudaError_t launch_decode(DecodeArgs& a, cudaStream_t stream, const char** err) {
-    return a.group <= 8 ? launch_decode<D, kE4M3, 1>(a, stream, err) : launch_decode<D, kE4M3, 2>(a, stream, err);
+cudaError_t launch_decode(DecodeArgs& a, cudaStream_t stream) {
+    return a.group <= 8 ? launch_decode<D, kE4M3, 1>(a, stream) : launch_decode<D, kE4M3, 2>(a, stream);
+}
+
+template <int D, bool kE4M3, int R>
+int64_t decode_work(const DecodeArgs& a) {
+    using Cfg = DecodeCfg<D, kE4M3, R>;
+    const int64_t items = static_cast<int64_t>(a.batch) * a.c.heads_kv * ((a.group + Cfg::kRows - 1) / Cfg::kRows);
+    return ((decode_keys(a) + Cfg::kSlice - 1) / Cfg::kSlice + kItemCost) * items;
 }
 
 }  // namespace
+
+bool decode_work_fits(const DecodeArgs& a, int32_t head_dim, int32_t kv_dtype) {
+    auto work = [&](auto one, auto two) { return a.group <= 8 ? one(a) : two(a); };
+    int64_t n;
+    if (kv_dtype == ODF_DTYPE_E4M3)
+        n = head_dim == 64 ? work(decode_work<64, true, 1>, decode_work<64, true, 2>)
+                           : work(decode_work<128, true, 1>, decode_work<128, true, 2>);
+    else
+        n = head_dim == 64 ? work(decode_work<64, false, 1>, decode_work<64, false, 2>)
+                           : work(decode_work<128, false, 1>, decode_work<128, false, 2>);
+    return n <= 0x7fffffffLL;
+}
 
 cudaError_t set_paged_kernel_attrs() {
     auto set = [](auto kernel, int bytes) {
@@ -1162,14 +1182,12 @@ int launch_paged_decode(DecodeArgs& a, int32_t head_dim, int32_t kv_dtype, cudaS
     a.v16_page = static_cast<uint32_t>(a.c.v_page / 16);
     a.v16_head = static_cast<uint32_t>(a.c.v_head / 16);
     a.v16_slot = static_cast<uint32_t>(a.c.v_slot / 16);
-    *err = nullptr;
     cudaError_t e;
     if (kv_dtype == ODF_DTYPE_E4M3)
-        e = head_dim == 64 ? launch_decode<64, true>(a, stream, err) : launch_decode<128, true>(a, stream, err);
+        e = head_dim == 64 ? launch_decode<64, true>(a, stream) : launch_decode<128, true>(a, stream);
     else
-        e = head_dim == 64 ? launch_decode<64, false>(a, stream, err) : launch_decode<128, false>(a, stream, err);
+        e = head_dim == 64 ? launch_decode<64, false>(a, stream) : launch_decode<128, false>(a, stream);
     if (e == cudaSuccess) return ODF_OK;
-    if (*err != nullptr) return ODF_ERR_UNSUPPORTED;
     *err = cudaGetErrorString(e);
     return ODF_ERR_CUDA;
 }

@@ -56,9 +56,12 @@ typedef struct odf_paged_cache {
  * with mod the ALiBi term slope[h] * (j - p) and the soft-cap of odf_fwd_params.  lens[b] <= 0
  * writes o = 0, lse = -inf.  K and V of keys that are not visible, and slots past a sequence's
  * end, may hold anything, NaN included.  Accumulation and softmax are fp32.
- * Limits (ODF_ERR_UNSUPPORTED past them): K pages, and V pages, of one layer span at most 64 GB; batch x
- * kv-heads x the table's room is at most 2^31 slices of 16 keys; 256 explicit slopes.  Lengths must not change
- * while a call runs.  Results do not depend on timing: the same call gives the same bits.
+ * Limits (ODF_ERR_UNSUPPORTED past them): K pages, and V pages, of one layer span at most 64 GB; 256 explicit
+ * slopes; batch below 2^23, heads_q below 2^16, batch x heads_q below 2^31; and
+ *   (ceil(keys / S) + 12) x batch x heads_kv x ceil(heads_q / heads_kv / T)  is below 2^31,
+ * with keys = max_pages * page_size (with a window at most window + sinks), S = 16 where a row of the cache has 256
+ * bytes and 32 where it has fewer, T = 8 up to eight query heads to a kv-head and 16 from nine on.  Lengths must not
+ * change while a call runs.  Results do not depend on timing: the same call gives the same bits.
  */
 typedef struct odf_decode_params {
     const void* q;              /* bf16 [batch, heads_q, head_dim] */
