@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
-#include <new>
+#include <exception>
 #include <vector>
 
 #include "paged_internal.h"
@@ -91,6 +91,37 @@ int view_of(const odf_paged_cache* c, bool tables, odf::PagedView* out) {
     out->table = c->page_table;
     out->table_stride = c->table_stride != 0 ? c->table_stride : c->max_pages;
     out->max_pages = static_cast<int32_t>(c->max_pages);
+    return ODF_OK;
+}
+
+// Ids of page copies, in order: inside the cache, no page written twice, none both read and written.  A few
+// pairs are compared with one another, many by a byte per page of the cache.
+int check_pairs(const int32_t* ids, int64_t n_pairs, int64_t num_pages) {
+    constexpr int64_t kFew = 32;
+    const char* twice = "a page is written twice";
+    const char* read = "a written page is also read";
+    std::vector<uint8_t> role;  // 1 = read, 2 = written
+    if (n_pairs > kFew) {
+        try {
+            role.resize(static_cast<size_t>(num_pages), 0);
+        } catch (const std::exception&) {
+            return set_error(ODF_ERR_UNSUPPORTED, "out of host memory");
+        }
+    }
+    for (int64_t i = 0; i < 2 * n_pairs; ++i) {
+        const int32_t id = ids[i];
+        if (id < 0 || id >= num_pages) return set_error(ODF_ERR_INVALID_ARG, "a page id is outside the cache");
+        if (n_pairs > kFew) {
+            if ((i & 1) && role[id] == 2) return set_error(ODF_ERR_INVALID_ARG, twice);
+            role[id] |= (i & 1) ? 2 : 1;
+            if (role[id] == 3) return set_error(ODF_ERR_INVALID_ARG, read);
+        } else {
+            for (int64_t j = 0; j < i; ++j) {
+                if (ids[j] != id || (~i & ~j & 1)) continue;
+                return set_error(ODF_ERR_INVALID_ARG, (i & j & 1) ? twice : read);
+            }
+        }
+    }
     return ODF_OK;
 }
 
@@ -266,20 +297,8 @@ int odf_page_copy_sm100(const odf_page_copy_params* p, void* stream) {
             if (s <= 0 || s > (int64_t{1} << 48) || (s * es) % 16 != 0)
                 return set_error(ODF_ERR_INVALID_ARG, "layer strides must be positive multiples of 16 bytes");
     }
-    try {  // 1 = read, 2 = written
-        std::vector<uint8_t> role(static_cast<size_t>(p->n_pairs > 0 ? p->cache.num_pages : 0), 0);
-        for (int64_t i = 0; i < 2 * p->n_pairs; ++i) {
-            const int32_t id = p->pairs[i];
-            if (id < 0 || id >= p->cache.num_pages) return set_error(ODF_ERR_INVALID_ARG, "a page id is outside the cache");
-            const uint8_t r = (i & 1) ? 2 : 1;
-            if ((i & 1) && role[id] == 2) return set_error(ODF_ERR_INVALID_ARG, "a page is written twice");
-            role[id] |= r;
-            if (role[id] == 3) return set_error(ODF_ERR_INVALID_ARG, "a written page is also read");
-        }
-    } catch (const std::bad_alloc&) {
-        return set_error(ODF_ERR_UNSUPPORTED, "out of host memory");
-    }
-    if (p->n_pairs == 0) return ODF_OK;
+    rc = check_pairs(p->pairs, p->n_pairs, p->cache.num_pages);
+    if (rc != ODF_OK || p->n_pairs == 0) return rc;
     int* status = nullptr;
     int sm_count = 0;
     rc = current_device_ready(&status, &sm_count);

@@ -8,7 +8,7 @@
  * pass in odf_sm100.h: same statuses, score mods, GQA rule (kv_head = q_head / group), softmax and
  * LSE definition, and the same rules for calls: plain pointers and sizes, nothing throws, device
  * calls are asynchronous on `stream` (a cudaStream_t; NULL = legacy default stream), allocate
- * nothing and read nothing back, so they can be captured into a CUDA graph after a first call.
+ * no device memory and read nothing back, so they can be captured into a CUDA graph after a first call.
  * The reference has no key-value cache; there is no counterpart to cite.
  *
  * Page ids and lengths live on the device, where the host cannot check them.  The kernels check
@@ -112,7 +112,8 @@ int odf_paged_append_sm100(const odf_append_params* p, void* stream);
  * Copies pages pairs[2i] -> pairs[2i + 1] (HOST array of n_pairs pairs, copied into the launch) of
  * K and V in every one of `layers` layers, layer l at k_pages + l * k_layer_stride elements.  Every
  * id must be in [0, num_pages), no page may be written twice, and no written page may also be read
- * (ODF_ERR_INVALID_ARG otherwise).  n_pairs == 0 does nothing.  The cache's tables, scales and
+ * (ODF_ERR_INVALID_ARG otherwise; the check of more than 32 pairs takes num_pages bytes of host memory, which are
+ * freed before the call returns).  n_pairs == 0 does nothing.  The cache's tables, scales and
  * page contents outside the written pages are not touched.
  */
 typedef struct odf_page_copy_params {
