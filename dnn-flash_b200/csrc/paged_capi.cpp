@@ -14,14 +14,14 @@ using odf::set_error;
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-int current_device_ready(int** status, int* sm_count) {
+int current_device_ready(int** status, int* sm_count = nullptr) {
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess) return set_error(ODF_ERR_NO_DEVICE, "no CUDA device");
     const char* err = "";
     const int rc = odf::ensure_device_ready(device, &err);
     if (rc != ODF_OK) return set_error(rc, err);
     *status = odf::device_status_ptr(device);
-    *sm_count = odf::device_sm_count(device);
+    if (sm_count != nullptr) *sm_count = odf::device_sm_count(device);
     return ODF_OK;
 }
 
@@ -276,6 +276,7 @@ int odf_paged_append_sm100(const odf_append_params* p, void* stream) {
     a.counts = p->counts;
     a.batch = static_cast<int32_t>(p->batch);
     a.tokens = static_cast<int32_t>(p->tokens);
+    a.sm_count = sm_count;
     const char* err = "";
     rc = odf::launch_paged_append(a, static_cast<int32_t>(p->cache.head_dim), p->cache.kv_dtype,
                                   static_cast<cudaStream_t>(stream), &err);
@@ -300,8 +301,7 @@ int odf_page_copy_sm100(const odf_page_copy_params* p, void* stream) {
     rc = check_pairs(p->pairs, p->n_pairs, p->cache.num_pages);
     if (rc != ODF_OK || p->n_pairs == 0) return rc;
     int* status = nullptr;
-    int sm_count = 0;
-    rc = current_device_ready(&status, &sm_count);
+    rc = current_device_ready(&status);
     if (rc != ODF_OK) return rc;
     odf::CopyArgs a;
     std::memset(&a, 0, sizeof(a));

@@ -54,7 +54,7 @@ struct AppendArgs {
     int64_t k_b, k_h, k_t, v_b, v_h, v_t;  // elements
     const int32_t* starts;
     const int32_t* counts;
-    int32_t batch, tokens;
+    int32_t batch, tokens, sm_count;
     FastDiv fd_tokens, fd_heads;
 };
 

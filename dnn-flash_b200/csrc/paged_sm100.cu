@@ -1198,7 +1198,7 @@ template <int D, bool kE4M3>
 void launch_append(const AppendArgs& a, int64_t rows, cudaStream_t stream) {
     constexpr int64_t kRowsPer = kAppendThreads / (D / 8);
     const int64_t wide = (rows + kRowsPer * kAppendUnroll - 1) / (kRowsPer * kAppendUnroll);
-    if (wide >= 148)
+    if (wide >= a.sm_count)
         paged_append_kernel<D, kE4M3, kAppendUnroll><<<static_cast<unsigned>(wide), kAppendThreads, 0, stream>>>(a);
     else
         paged_append_kernel<D, kE4M3, 1>
