@@ -601,7 +601,8 @@ def _outputs(q, out, lse_out, out_dtype, want_lse, *lead):
 
 
 def _clip(n):
-    """A count as the C side takes it: below zero is refused there, and past 63 bits nothing changes."""
+    """A count (or a sequence of a pool) as the C side takes it, where an integer past 64 bits would wrap: below zero
+    it is refused there, and past 63 bits no count changes and no sequence is found."""
     return max(-1, min(n, _INT64_MAX))
 
 
@@ -748,7 +749,7 @@ class PagePool:
     def __init__(self, num_pages: int, page_size: int):
         self._lib = load_library()
         self._pool = C.c_void_p()
-        _check(self._lib.odf_page_pool_create(num_pages, page_size, C.byref(self._pool)))
+        _check(self._lib.odf_page_pool_create(_clip(num_pages), _clip(page_size), C.byref(self._pool)))
         self.num_pages, self.page_size = num_pages, page_size
 
     def __del__(self):
@@ -765,22 +766,22 @@ class PagePool:
     def fork(self, seq: int) -> int:
         """A new sequence with the same tokens; every page is shared until one of the two writes it."""
         child = C.c_int64()
-        _check(self._lib.odf_page_pool_fork(self._pool, seq, C.byref(child)))
+        _check(self._lib.odf_page_pool_fork(self._pool, _clip(seq), C.byref(child)))
         return child.value
 
     def extend(self, seq: int, tokens: int) -> list[tuple[int, int]]:
         """Room for ``tokens`` more tokens; raises OdfError(ODF_ERR_NO_PAGES), changing nothing, without it."""
         pair, n = (C.c_int32 * 2)(), C.c_int64()
-        _check(self._lib.odf_page_pool_extend(self._pool, seq, tokens, pair, C.byref(n)))
+        _check(self._lib.odf_page_pool_extend(self._pool, _clip(seq), _clip(tokens), pair, C.byref(n)))
         return [(pair[0], pair[1])] if n.value else []
 
     def truncate(self, seq: int, length: int) -> None:
         """Drops the tokens past ``length``."""
-        _check(self._lib.odf_page_pool_truncate(self._pool, seq, length))
+        _check(self._lib.odf_page_pool_truncate(self._pool, _clip(seq), _clip(length)))
 
     def free(self, seq: int) -> None:
         """Ends a sequence."""
-        _check(self._lib.odf_page_pool_free(self._pool, seq))
+        _check(self._lib.odf_page_pool_free(self._pool, _clip(seq)))
 
     def compact(self) -> list[tuple[int, int]]:
         """Moves pages so that the used ones are the first ones."""
@@ -791,14 +792,14 @@ class PagePool:
 
     def length(self, seq: int) -> int:
         tokens, pages = C.c_int64(), C.c_int64()
-        _check(self._lib.odf_page_pool_length(self._pool, seq, C.byref(tokens), C.byref(pages)))
+        _check(self._lib.odf_page_pool_length(self._pool, _clip(seq), C.byref(tokens), C.byref(pages)))
         return tokens.value
 
     def pages(self, seq: int) -> list[int]:
         tokens, pages = C.c_int64(), C.c_int64()
-        _check(self._lib.odf_page_pool_length(self._pool, seq, C.byref(tokens), C.byref(pages)))
+        _check(self._lib.odf_page_pool_length(self._pool, _clip(seq), C.byref(tokens), C.byref(pages)))
         ids = (C.c_int32 * max(pages.value, 1))()
-        _check(self._lib.odf_page_pool_table(self._pool, seq, ids, pages.value))
+        _check(self._lib.odf_page_pool_table(self._pool, _clip(seq), ids, pages.value))
         return list(ids[:pages.value])
 
     def table(self, seqs, max_pages: int | None = None):
