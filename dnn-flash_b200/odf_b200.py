@@ -743,7 +743,8 @@ class PagePool:
     """Which pages of a cache are free, and every sequence's table (odf_page_pool_*; host only).
 
     ``extend`` and ``compact`` return (source, destination) pairs for ``page_copy``, to be run before the
-    cache is written or the pool changed again.  Not thread-safe.
+    cache is written.  Pairs of consecutive calls of ``extend`` may go into one copy, which has to run before any
+    other call that changes the pool (``fork``, ``truncate``, ``free``, ``compact``).  Not thread-safe.
     """
 
     def __init__(self, num_pages: int, page_size: int):

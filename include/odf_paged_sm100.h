@@ -129,7 +129,9 @@ int odf_page_copy_sm100(const odf_page_copy_params* p, void* stream);
  * Host-side page pool: which pages are free, how many sequences share each, and every sequence's
  * table.  No CUDA calls.  Not thread-safe: one pool is used by one thread at a time.  Copies that a
  * call asks for come back as (source, destination) pairs, which the caller hands to
- * odf_page_copy_sm100 before it writes the cache again.
+ * odf_page_copy_sm100 before it writes the cache again.  The pairs of consecutive calls of extend may be
+ * gathered into one copy; it has to run before any other call that changes the pool (fork, truncate, free, compact),
+ * which may hand out a page that a pair still reads.
  */
 typedef struct odf_page_pool odf_page_pool;
 
