@@ -59,7 +59,8 @@ __device__ __forceinline__ Visible visible_keys(const DecodeArgs& a, int len) {
 // want 128 rows of keys by 8 columns through tensor memory; the warp-level product leaves the tensor
 // pipe 9% busy (16% with an 8-bit cache) and needs no hand-over between warps.
 //
-// 64 sequences of up to 8192 keys, 64/8 heads: 1075 MB in 163 us, 6.6 TB/s; one of 129 keys 4.3 us.
+// 64 sequences of up to 8192 keys, 64/8 heads, three draws of their lengths: 1079, 1132 and 1131 MB of visible keys
+// in 165, 172 and 176 us (6.4 to 6.6 TB/s); one sequence of 129 keys 4.5 us in a replayed graph.
 //
 // Work: an item is (sequence, kv-head, block of query heads); its visible keys are cut into slices of 16 or
 // 32.  The slices of all items in a row are dealt to the CTAs in equal consecutive runs, whatever
@@ -97,8 +98,8 @@ struct DecodeCfg {
     static constexpr int kSlice = kRowBytes >= 256 ? 16 : 32;
     static constexpr int kTileBytes = kSlice * kRowBytes;   // K or V of a slice
     static constexpr int kStageBytes = 2 * kTileBytes;
-    // 16 KB a warp with three CTAs of four warps on an SM, 24 KB with two: 96 or 128 KB of loads in flight
-    // behind the slices that are being computed.  Three do as well or better wherever their registers
+    // 16 KB a warp with three CTAs of four warps on an SM, 24 KB with two: 96 or 128 KB of loads in flight on an SM
+    // (144 or 160 with 8-bit rows of 64) behind the slices that are being computed.  Three do as well or better wherever their registers
     // allow it (64 ragged sequences of 8-bit rows of 64: 57 us against 66).
     static constexpr int kCtas = R == 1 ? kCtasPerSm : 2;
     static constexpr int kStages = (kCtas == 3 ? 16384 : 24576) / kStageBytes;

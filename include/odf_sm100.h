@@ -131,7 +131,7 @@ size_t odf_fwd_workspace_size(const odf_fwd_params* p);
 typedef struct odf_window {
     int64_t window;    /* >= 1 */
     int64_t sinks;     /* >= 0 */
-    int64_t q_offset;  /* >= 0; q_offset + seqlen_q below 2^31 */
+    int64_t q_offset;  /* >= 0; q_offset + seqlen_q at most 2^31 - 257 */
 } odf_window;
 
 int odf_flash_fwd_window_sm100(const odf_fwd_params* p, const odf_window* w, void* stream);
